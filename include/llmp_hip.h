@@ -418,6 +418,94 @@ int llmp_attn_block(uint64_t handle, int layer, int position, uint64_t d_positio
 int llmp_attn_block_batch(uint64_t handle, int layer, int pos0, int n_tokens, uint64_t x,
                           uint64_t stream);
 
+/* ---- a batch of sequences over one paged pool ---------------------------------------------
+ * The reference keeps one KV cache per conversation and runs sequences one after the other
+ * (LLMEngine.java:400-421, ConversationCache.java:36-56).  Here many sequences share one pool of
+ * pages, a prefix that they have in common is stored and attended once, and one call serves all of
+ * their tokens.  Everything that changes from step to step (lengths, block tables, positions, slots)
+ * is device memory, so a step captured once (llmp_graph_*) replays as the sequences grow.
+ *
+ * Arrays, all int32 on the device, for n_seqs sequences and W = ceil(max_seq / page_size):
+ *   blocks     [n_seqs][W]   page of each block of page_size positions of each sequence
+ *   seq_start  [n_seqs + 1]  first token of each sequence in the step's arrays; [n_seqs]: their number
+ *   positions  [n_tokens]    position of each token in its sequence (-1: no token)
+ *   slots      [n_tokens]    where its row is stored: page * page_size + row (-1: nowhere)
+ * A page or slot outside the pool is never touched: such a block holds no rows, such a token stores
+ * none.  A position outside [0, max_seq) is no token. */
+
+/* A handle for sequences of up to max_seq rows in a pool of n_pages pages of page_size (16, 32, 64,
+ * 128 or 256) rows; head_dim 64, 96, 128 or 256; any GQA group; dtype an LLMP_KV_* type.  The pool
+ * itself is the caller's memory (llmp_paged_bind).  llmp_layer_config, llmp_layer_sinks,
+ * llmp_layer_norm_mode, llmp_rope_upload (tables of max_seq rows) and llmp_kv_destroy take the handle;
+ * the calls of a contiguous cache refuse it, as those below refuse a contiguous cache's.  One owner:
+ * calls on one handle must not overlap, replays of graphs captured with it included. */
+int llmp_paged_create(int n_layers, int n_pages, int page_size, int max_seq, int n_kv_heads,
+                      int head_dim, int dtype, uint64_t *handle);
+/* Bytes of the handle's pool: per layer K pages [page][kv_head][row][head_dim] (fp32, or int8 quants
+ * and then their scales [page][kv_head][row][head_dim/32] fp32), then V the same, each of these
+ * padded to 256 bytes. */
+int llmp_paged_bytes(uint64_t handle, uint64_t *bytes);
+/* Use `pool` (device memory of that size, 256-byte aligned, of any content) from the next call on. */
+int llmp_paged_bind(uint64_t handle, uint64_t pool);
+/* Device addresses of one layer's planes in the bound pool (scales 0 for fp32).  Any out may be NULL. */
+int llmp_paged_planes(uint64_t handle, int layer, uint64_t *k, uint64_t *k_scales, uint64_t *v,
+                      uint64_t *v_scales);
+
+/* The tables of one step, from the sequences' lengths (up to 8192 sequences).
+ *   len [n_seqs]   rows that each sequence has in the pool
+ *   grow [n_seqs]  its new tokens in this step (0 or more), or below 0: the sequence has ended
+ *   free_pages [n_pages], n_free [1]   a stack of free pages and their number
+ *   blocks [n_seqs][W]  in and out: the blocks of `len` rows are given
+ * First the blocks from shared_blocks on (those before belong to a prefix that others use) of the
+ * ended sequences are pushed on the stack, in order of sequence and block; then each other sequence's
+ * missing blocks for len + grow rows are popped from its top, in the same order.  Results: blocks,
+ * free_pages, n_free_out [1], len_out [n_seqs] (len + grow, 0 for an ended one), seq_start, positions
+ * and slots of the new tokens (-1 from there to max_tokens).  len_out may be len and n_free_out may be
+ * n_free; no other arrays may overlap.  Entries that no result names are left as they were.
+ * status [1]: 0; a positive number: so many pages were missing; -1: a length below 0 or above max_seq,
+ * or more free pages than the pool has; -2: more than max_tokens new tokens.  A step with another
+ * status than 0 changes no block, page or length and has no tokens (seq_start all 0, positions and
+ * slots all -1), so calls that follow it in a graph do nothing. */
+int llmp_paged_tables(uint64_t handle, int n_seqs, int shared_blocks, int max_tokens, uint64_t len,
+                      uint64_t grow, uint64_t free_pages, uint64_t n_free, uint64_t blocks,
+                      uint64_t len_out, uint64_t n_free_out, uint64_t seq_start, uint64_t positions,
+                      uint64_t slots, uint64_t status, uint64_t stream);
+
+/* Rotary positions, QK-norm and the append of a step's tokens.  Token t's query row (n_heads*head_dim
+ * elements at q + t*q_stride elements) is normed if the layer has QK-norm and rotated by its position
+ * with the layer's table (llmp_rope_upload: interleaved or half layout, part of the head, linear or
+ * YaRN scaling are all the table's and llmp_layer_config's), and written to q_out as fp32; its K row is
+ * treated likewise and stored with its V row at slots[t], in a contiguous cache's decode arithmetic:
+ * the stored rows equal llmp_attn_decode's bit for bit (Q8_0 pools: its quantiser).
+ * k = v = 0: only the queries (slots may be 0).  in_type: the type of q, k and v (LLMP_IN_*); strides
+ * in elements, at least a row; q_out may be q for fp32 at equal strides.  A token with no position is
+ * skipped, its q_out row too.  No two tokens may name one slot. */
+#define LLMP_IN_F32  0
+#define LLMP_IN_BF16 1
+int llmp_paged_append(uint64_t handle, int layer, int n_tokens, uint64_t positions, uint64_t slots,
+                      int in_type, uint64_t q, int64_t q_stride, uint64_t k, int64_t k_stride,
+                      uint64_t v, int64_t v_stride, uint64_t q_out, int64_t out_stride,
+                      uint64_t stream);
+
+/* Attention of a step's tokens (queries from llmp_paged_append, fp32, 16-byte aligned, strides
+ * multiples of 4): token t of sequence b attends rows [start, positions[t]] of its sequence (start by
+ * the layer's window), its own among them, with the layer's scale, soft-cap and sinks, and the optional
+ * gate (fp32 [n_tokens][n_heads*head_dim], 0 = none) as llmp_attn_decode_ex applies it.
+ * The rows [0, prefix_len) are the same for every sequence: they are taken from sequence 0's blocks and
+ * read once for all tokens, whatever the other sequences' blocks there say.  prefix_len 0 shares
+ * nothing.  max_len: a bound of the sequences' lengths (0: max_seq); it sets how the work is divided
+ * and changes no result beyond the order of its sums.
+ * Tokens of one sequence are consecutive; n_tokens is the size of the arrays, and rows of `out` from
+ * token seq_start[n_seqs] on are left as they were.  A token with nothing to attend gives zeros.
+ * Precision as llmp_attn_prefill_f32's, whatever the magnitudes in the pool.  A row that holds an
+ * infinity or NaN spoils the outputs of the tokens that attend it and no others.
+ * The call's workspace (prefix and own splits * n_tokens * n_heads * (head_dim + 2) floats) grows with
+ * the handle; a captured call needs one of its size to have run before, and keeps what it uses. */
+int llmp_paged_attn(uint64_t handle, int layer, int n_seqs, int n_tokens, int prefix_len, int max_len,
+                    uint64_t seq_start, uint64_t positions, uint64_t blocks, uint64_t q,
+                    int64_t q_stride, uint64_t gate, uint64_t out, int64_t out_stride,
+                    uint64_t stream);
+
 /* ---- profiling (the reference's -Dcuda.profile section timers,
  *      CudaForwardPass.java:1646-1737, as HIP events around each kernel) ------------------ */
 #define LLMP_PROF_DECODE_SPLIT   0  /* split-K decode kernel (QK-norm, RoPE, append, QK/softmax/PV;

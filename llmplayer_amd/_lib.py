@@ -33,10 +33,11 @@ LLMP_GGML_IQ3_XXS, LLMP_GGML_IQ3_S, LLMP_GGML_IQ2_S = 18, 21, 22
 (LLMP_W_ATTN_NORM, LLMP_W_Q, LLMP_W_K, LLMP_W_V, LLMP_W_QKV, LLMP_W_O, LLMP_W_Q_BIAS, LLMP_W_K_BIAS,
  LLMP_W_V_BIAS, LLMP_W_O_BIAS, LLMP_W_POST_ATTN_NORM) = range(11)
 LLMP_INPUT_F32, LLMP_INPUT_Q8_1 = 0, 1
+LLMP_IN_F32, LLMP_IN_BF16 = 0, 1
 LLMP_PROF_DECODE_SPLIT, LLMP_PROF_DECODE_REDUCE = 0, 1
 LLMP_PROF_PREFILL_APPEND, LLMP_PROF_PREFILL_ATTN = 2, 3
 
-_u64, _i32, _f32 = C.c_uint64, C.c_int, C.c_float
+_u64, _i64, _i32, _f32 = C.c_uint64, C.c_int64, C.c_int, C.c_float
 _pu64 = C.POINTER(C.c_uint64)
 _pf = C.POINTER(C.c_float)
 _vp = C.c_void_p
@@ -93,6 +94,15 @@ SIGNATURES = {
     "llmp_attn_prefill_shared_f32": [_u64, _i32, _i32, _i32, _i32, _u64, _u64, _u64, _u64],
     "llmp_decode_plan": [_u64, _i32, _i32, _i32, C.POINTER(_i32), C.POINTER(_i32),
                          C.POINTER(_i32), C.POINTER(_i32)],
+    "llmp_paged_create": [_i32] * 7 + [_pu64],
+    "llmp_paged_bytes": [_u64, _pu64],
+    "llmp_paged_bind": [_u64, _u64],
+    "llmp_paged_planes": [_u64, _i32, _pu64, _pu64, _pu64, _pu64],
+    "llmp_paged_tables": [_u64, _i32, _i32, _i32] + [_u64] * 12,
+    "llmp_paged_append": [_u64, _i32, _i32, _u64, _u64, _i32, _u64, _i64, _u64, _i64, _u64, _i64, _u64,
+                          _i64, _u64],
+    "llmp_paged_attn": [_u64, _i32, _i32, _i32, _i32, _i32, _u64, _u64, _u64, _u64, _i64, _u64, _u64,
+                        _i64, _u64],
     "llmp_graph_begin": [_u64],
     "llmp_graph_end": [_u64, _pu64],
     "llmp_graph_launch": [_u64, _u64],

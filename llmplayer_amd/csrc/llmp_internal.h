@@ -107,6 +107,20 @@ hipError_t launch_prefill_combine(const pk::PrefillArgs& a, int head_dim, int ks
 hipError_t launch_prefill_wide(const pk::PrefillArgs& a, int head_dim, int group, void* ws, int tile0, int n_tiles,
                                int row_end, int n_cu, hipStream_t stream);
 
+namespace pg {
+struct TablesArgs;
+struct AppendArgs;
+struct AttnArgs;
+}
+// A batch of sequences over a paged pool (paged_kernels.h, paged_attn_kernels.h): the tables of a
+// step, the append of its tokens, and its attention: partials of the prefix rows (own = false) or of
+// each sequence's own rows with 16*mt query rows a workgroup (mt 1, 2, and 4 up to head_dim 128),
+// joined by the combine.
+hipError_t launch_paged_tables(const pg::TablesArgs& a, hipStream_t stream);
+hipError_t launch_paged_append(const pg::AppendArgs& a, int head_dim, hipStream_t stream);
+hipError_t launch_paged_attn(const pg::AttnArgs& a, int head_dim, bool q8, bool own, int mt, hipStream_t stream);
+hipError_t launch_paged_combine(const pg::AttnArgs& a, int head_dim, hipStream_t stream);
+
 // Plain 16-byte-per-thread copy kernel.
 hipError_t launch_copy(void* dst, const void* src, size_t bytes, hipStream_t stream);
 

@@ -6,6 +6,8 @@
 #include "prefill_kernels.h"
 #include "gemv_kernels.h"
 #include "proj_gemm_kernels.h"
+#include "paged_args.h"
+#include "paged_plan.h"
 #include "workspace.h"
 
 #include <algorithm>
@@ -109,6 +111,12 @@ struct KvHandle {
     void* blkb_buf = nullptr;        // token-batched block scratch (llmp_attn_block_batch)
     size_t blkb_bytes = 0;
     size_t part_slots = 0;    // (split, query head) slots the workspace holds
+    // A paged pool (llmp_paged_create): no rows of its own, max_seq the longest sequence.
+    bool paged = false;
+    int n_pages = 0, page_shift = 0;
+    char* bound = nullptr;           // the caller's pool (llmp_paged_bind)
+    int* ticket = nullptr;           // llmp_paged_tables: zero between calls
+    Workspace paged_ws;              // partials of llmp_paged_attn
     bool prof_on = false;
     std::vector<ProfPair> prof_pending[LLMP_PROF_KINDS];
     std::vector<hipEvent_t> prof_free;
@@ -142,6 +150,20 @@ struct KvHandle {
         return q8() ? (size_t)n_layers * q8_layer_bytes()
                     : 2 * (size_t)n_layers * plane_floats * sizeof(float);
     }
+    // A paged pool, per layer: K pages, K scales, V pages, V scales (Q8_0), each padded as above.
+    size_t paged_plane_bytes() const { return q8() ? q8_quant_bytes() : pad256(plane_floats * sizeof(float)); }
+    size_t paged_layer_bytes() const { return 2 * (paged_plane_bytes() + (q8() ? q8_scale_bytes() : 0)); }
+    pg::PoolPlanes paged_planes(int layer) const {
+        char* k = bound + (size_t)layer * paged_layer_bytes();
+        char* v = k + paged_layer_bytes() / 2;
+        float* ks = q8() ? reinterpret_cast<float*>(k + paged_plane_bytes()) : nullptr;
+        float* vs = q8() ? reinterpret_cast<float*>(v + paged_plane_bytes()) : nullptr;
+        return {k, ks, v, vs, n_pages, page_shift, n_kv_heads};
+    }
+    PagedShape paged_shape() const {
+        return {n_layers, n_pages, 1 << page_shift, max_seq, n_kv_heads, head_dim, dtype};
+    }
+    int paged_width() const { return (int)paged_shape().width(); }
     // Range exponents of the stored rows (dk::note_range), [layer][kv_head][K, V] int32, after
     // the rows in the same allocation: zeroed with them, raised by every append and by
     // llmp_kv_write / llmp_kv_write_q8.
@@ -202,7 +224,18 @@ KvHandle* find_handle(uint64_t h) {
 
 #define LLMP_GET_HANDLE(var, h)                                                   \
     KvHandle* var = find_handle(h);                                               \
+    if (!var) return fail(LLMP_ERR_BAD_HANDLE, "unknown KV handle %llu", (unsigned long long)(h)); \
+    if (var->paged)                                                               \
+    return fail(LLMP_ERR_INVALID_ARG, "handle %llu is a paged pool's", (unsigned long long)(h))
+
+// The set-up calls that a paged pool's handle takes too, and the calls that take nothing else.
+#define LLMP_GET_ANY_HANDLE(var, h)                                               \
+    KvHandle* var = find_handle(h);                                               \
     if (!var) return fail(LLMP_ERR_BAD_HANDLE, "unknown KV handle %llu", (unsigned long long)(h))
+#define LLMP_GET_PAGED(var, h)                                                    \
+    LLMP_GET_ANY_HANDLE(var, h);                                                  \
+    if (!var->paged)                                                              \
+    return fail(LLMP_ERR_INVALID_ARG, "handle %llu is not a paged pool's", (unsigned long long)(h))
 
 void free_handle(KvHandle* kv) {
     if (kv->pool) (void)hipFree(kv->pool);
@@ -219,12 +252,13 @@ void free_handle(KvHandle* kv) {
     }
     if (kv->blk_buf) (void)hipFree(kv->blk_buf);
     if (kv->blkb_buf) (void)hipFree(kv->blkb_buf);
-    for (Workspace* w : {&kv->prefill_ws, &kv->prefill_part, &kv->wide_ws, &kv->many_buf})
+    for (Workspace* w : {&kv->prefill_ws, &kv->prefill_part, &kv->wide_ws, &kv->many_buf, &kv->paged_ws})
         if (w->mem) (void)hipFree(w->mem);
     for (void* p : kv->outgrown) (void)hipFree(p);
     if (kv->part_o) (void)hipFree(kv->part_o);
     if (kv->part_ml) (void)hipFree(kv->part_ml);
     if (kv->done) (void)hipFree(kv->done);
+    if (kv->ticket) (void)hipFree(kv->ticket);
     for (auto& v : kv->prof_pending)
         for (auto& p : v) {
             (void)hipEventDestroy(p.begin);
@@ -943,7 +977,7 @@ int llmp_rope_table_yarn(int rope_dim, int max_seq, float theta, const float* fr
 int llmp_rope_upload(uint64_t handle, int which, const float* cos_t, const float* sin_t,
                      int max_seq, int half_rope) {
     if (int rc = ensure_init()) return rc;
-    LLMP_GET_HANDLE(kv, handle);
+    LLMP_GET_ANY_HANDLE(kv, handle);
     if (which != LLMP_ROPE_SEL_GLOBAL && which != LLMP_ROPE_SEL_LOCAL)
         return fail(LLMP_ERR_INVALID_ARG, "llmp_rope_upload: which=%d", which);
     if (!cos_t || !sin_t || half_rope <= 0 || 2 * half_rope > kv->head_dim || max_seq < kv->max_seq)
@@ -973,7 +1007,7 @@ int llmp_layer_config(uint64_t handle, int layer, int n_heads, int n_kv_heads, i
                       int rope_type, int rope_sel, int window, int is_global, float scale,
                       float softcap, float eps, const float* qnorm_w, const float* knorm_w) {
     if (int rc = ensure_init()) return rc;
-    LLMP_GET_HANDLE(kv, handle);
+    LLMP_GET_ANY_HANDLE(kv, handle);
     if (layer < 0 || layer >= kv->n_layers)
         return fail(LLMP_ERR_OUT_OF_RANGE, "layer %d outside [0, %d)", layer, kv->n_layers);
     if (n_kv_heads != kv->n_kv_heads || head_dim != kv->head_dim)
@@ -1000,7 +1034,7 @@ int llmp_layer_config(uint64_t handle, int layer, int n_heads, int n_kv_heads, i
     if ((qnorm_w == nullptr) != (knorm_w == nullptr))
         return fail(LLMP_ERR_INVALID_ARG, "layer %d: QK-norm needs both weights or neither", layer);
 
-    if ((size_t)kMaxSplits * (size_t)n_heads > kv->part_slots) {
+    if (!kv->paged && (size_t)kMaxSplits * (size_t)n_heads > kv->part_slots) {
         // More query heads than llmp_kv_create sized the split workspace for (groups above
         // kMaxGroup): it grows here, at set-up, so graphs captured before must be captured again.
         const size_t slots = (size_t)kMaxSplits * (size_t)n_heads;
@@ -1101,7 +1135,7 @@ int llmp_attn_decode_shared(uint64_t handle, int layer, int src_layer, int posit
 
 int llmp_layer_norm_mode(uint64_t handle, int layer, int mode) {
     if (int rc = ensure_init()) return rc;
-    LLMP_GET_HANDLE(kv, handle);
+    LLMP_GET_ANY_HANDLE(kv, handle);
     if (layer < 0 || layer >= kv->n_layers)
         return fail(LLMP_ERR_OUT_OF_RANGE, "layer %d outside [0, %d)", layer, kv->n_layers);
     if (mode & ~(LLMP_NORM_SEQUENTIAL | LLMP_NORM_V))
@@ -1724,7 +1758,7 @@ static int batch_pass(KvHandle* kv, int layer, int pos0, int K, float* xc, uint6
 
 int llmp_layer_sinks(uint64_t handle, int layer, const float* sinks) {
     if (int rc = ensure_init()) return rc;
-    LLMP_GET_HANDLE(kv, handle);
+    LLMP_GET_ANY_HANDLE(kv, handle);
     if (layer < 0 || layer >= kv->n_layers)
         return fail(LLMP_ERR_OUT_OF_RANGE, "layer %d outside [0, %d)", layer, kv->n_layers);
     LayerCfg& c = kv->layers[(size_t)layer];
@@ -1974,6 +2008,224 @@ static int enqueue_prefill(KvHandle* kv, int layer, int src_layer, int pos0, int
         LLMP_HIP_CHECK(hipEventRecord(e3, st), "hipEventRecord");
         kv->prof_pending[LLMP_PROF_PREFILL_ATTN].push_back({e2, e3});
     }
+    return LLMP_OK;
+}
+
+// ---- a batch of sequences over a paged pool --------------------------------------------------------
+int llmp_paged_create(int n_layers, int n_pages, int page_size, int max_seq, int n_kv_heads, int head_dim,
+                      int dtype, uint64_t* handle) {
+    if (int rc = ensure_init()) return rc;
+    if (!handle) return fail(LLMP_ERR_INVALID_ARG, "llmp_paged_create: null handle out");
+    const PagedShape shape{n_layers, n_pages, page_size, max_seq, n_kv_heads, head_dim, dtype};
+    PagedMessage msg;
+    if (int rc = paged_create_check(shape, msg)) return fail(rc, "%s", msg.text);
+    int shift = 4;
+    while ((1 << shift) != page_size) ++shift;
+    auto kv = std::make_unique<KvHandle>();
+    kv->paged = true;
+    kv->n_layers = n_layers;
+    kv->n_pages = n_pages;
+    kv->page_shift = shift;
+    kv->max_seq = max_seq;
+    kv->n_kv_heads = n_kv_heads;
+    kv->head_dim = head_dim;
+    kv->dtype = dtype;
+    kv->plane_floats = ((size_t)n_pages << shift) * (size_t)n_kv_heads * (size_t)head_dim;
+    kv->layers.resize((size_t)n_layers);
+    hipError_t e = hipMalloc(&kv->ticket, sizeof(int));
+    if (e == hipSuccess) e = hipMemset(kv->ticket, 0, sizeof(int));
+    if (e != hipSuccess) {
+        free_handle(kv.get());
+        return fail(e == hipErrorOutOfMemory ? LLMP_ERR_OUT_OF_MEMORY : LLMP_ERR_HIP, "llmp_paged_create: %s",
+                    hipGetErrorString(e));
+    }
+    std::lock_guard<std::mutex> lk(G().mu);
+    const uint64_t id = G().next_handle++;
+    G().handles[id] = std::move(kv);
+    *handle = id;
+    return LLMP_OK;
+}
+
+int llmp_paged_bytes(uint64_t handle, uint64_t* bytes) {
+    if (int rc = ensure_init()) return rc;
+    LLMP_GET_PAGED(kv, handle);
+    if (!bytes) return fail(LLMP_ERR_INVALID_ARG, "llmp_paged_bytes: null out");
+    *bytes = (uint64_t)kv->n_layers * kv->paged_layer_bytes();
+    return LLMP_OK;
+}
+
+int llmp_paged_bind(uint64_t handle, uint64_t pool) {
+    if (int rc = ensure_init()) return rc;
+    LLMP_GET_PAGED(kv, handle);
+    if (!pool || (pool & 255)) return fail(LLMP_ERR_INVALID_ARG, "llmp_paged_bind: null or not 256-byte aligned pool");
+    kv->bound = reinterpret_cast<char*>(pool);
+    return LLMP_OK;
+}
+
+int llmp_paged_planes(uint64_t handle, int layer, uint64_t* k, uint64_t* k_scales, uint64_t* v, uint64_t* v_scales) {
+    if (int rc = ensure_init()) return rc;
+    LLMP_GET_PAGED(kv, handle);
+    if (layer < 0 || layer >= kv->n_layers)
+        return fail(LLMP_ERR_OUT_OF_RANGE, "layer %d outside [0, %d)", layer, kv->n_layers);
+    if (!kv->bound) return fail(LLMP_ERR_INVALID_ARG, "llmp_paged_planes: no pool (llmp_paged_bind)");
+    const pg::PoolPlanes p = kv->paged_planes(layer);
+    if (k) *k = reinterpret_cast<uint64_t>(p.k);
+    if (v) *v = reinterpret_cast<uint64_t>(p.v);
+    if (k_scales) *k_scales = reinterpret_cast<uint64_t>(p.ks);
+    if (v_scales) *v_scales = reinterpret_cast<uint64_t>(p.vs);
+    return LLMP_OK;
+}
+
+int llmp_paged_tables(uint64_t handle, int n_seqs, int shared_blocks, int max_tokens, uint64_t len, uint64_t grow,
+                      uint64_t free_pages, uint64_t n_free, uint64_t blocks, uint64_t len_out, uint64_t n_free_out,
+                      uint64_t seq_start, uint64_t positions, uint64_t slots, uint64_t status, uint64_t stream) {
+    if (int rc = ensure_init()) return rc;
+    LLMP_GET_PAGED(kv, handle);
+    const uint64_t all[] = {len, grow, free_pages, n_free, blocks, len_out, n_free_out, seq_start, positions, slots, status};
+    PagedMessage msg;
+    if (int rc = paged_tables_check(kv->paged_shape(), n_seqs, shared_blocks, max_tokens, all, 11, msg))
+        return fail(rc, "%s", msg.text);
+    pg::TablesArgs a{};
+    a.n = n_seqs;
+    a.max_tokens = max_tokens;
+    a.shared = shared_blocks;
+    a.shift = kv->page_shift;
+    a.max_seq = kv->max_seq;
+    a.width = kv->paged_width();
+    a.n_pages = kv->n_pages;
+    a.len = reinterpret_cast<const int*>(len);
+    a.grow = reinterpret_cast<const int*>(grow);
+    a.free_pages = reinterpret_cast<int*>(free_pages);
+    a.n_free = reinterpret_cast<const int*>(n_free);
+    a.blocks = reinterpret_cast<int*>(blocks);
+    a.len_out = reinterpret_cast<int*>(len_out);
+    a.n_free_out = reinterpret_cast<int*>(n_free_out);
+    a.seq_start = reinterpret_cast<int*>(seq_start);
+    a.positions = reinterpret_cast<int*>(positions);
+    a.slots = reinterpret_cast<int*>(slots);
+    a.status = reinterpret_cast<int*>(status);
+    a.ticket = kv->ticket;
+    LLMP_HIP_CHECK(launch_paged_tables(a, pick_stream(stream)), "paged tables launch");
+    return LLMP_OK;
+}
+
+// A configured layer of a paged handle whose pool is bound.
+static int paged_layer(const KvHandle* kv, int layer, const char* what) {
+    if (layer < 0 || layer >= kv->n_layers)
+        return fail(LLMP_ERR_OUT_OF_RANGE, "layer %d outside [0, %d)", layer, kv->n_layers);
+    if (!kv->layers[(size_t)layer].configured)
+        return fail(LLMP_ERR_INVALID_ARG, "layer %d was never configured (llmp_layer_config)", layer);
+    if (!kv->bound) return fail(LLMP_ERR_INVALID_ARG, "%s: no pool (llmp_paged_bind)", what);
+    return LLMP_OK;
+}
+
+int llmp_paged_append(uint64_t handle, int layer, int n_tokens, uint64_t positions, uint64_t slots, int in_type,
+                      uint64_t q, int64_t q_stride, uint64_t k, int64_t k_stride, uint64_t v, int64_t v_stride,
+                      uint64_t q_out, int64_t out_stride, uint64_t stream) {
+    if (int rc = ensure_init()) return rc;
+    LLMP_GET_PAGED(kv, handle);
+    if (int rc = paged_layer(kv, layer, "llmp_paged_append")) return rc;
+    const LayerCfg& c = kv->layers[(size_t)layer];
+    const int D = kv->head_dim;
+    PagedMessage msg;
+    if (int rc = paged_append_check(kv->paged_shape(), c.n_heads, n_tokens, positions, slots, in_type, q, q_stride, k,
+                                    k_stride, v, v_stride, q_out, out_stride, msg))
+        return fail(rc, "%s", msg.text);
+    pg::AppendArgs a{};
+    if (c.rope_sel != LLMP_ROPE_SEL_NONE) {
+        const RopeTable& t = kv->rope[c.rope_sel];
+        if (!t.d_cos) return fail(LLMP_ERR_INVALID_ARG, "layer %d selects a RoPE table never uploaded", layer);
+        a.cos_t = t.d_cos;
+        a.sin_t = t.d_sin;
+        a.half_rope = t.half;
+    }
+    a.pool = kv->paged_planes(layer);
+    a.positions = reinterpret_cast<const int*>(positions);
+    a.slots = reinterpret_cast<const int*>(slots);
+    a.q = reinterpret_cast<const void*>(q);
+    a.k = reinterpret_cast<const void*>(k);
+    a.v = reinterpret_cast<const void*>(v);
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.out_stride = out_stride;
+    a.out = reinterpret_cast<float*>(q_out);
+    a.qnw = c.d_qnw;
+    a.knw = c.d_knw;
+    a.n_tokens = n_tokens;
+    a.n_heads = c.n_heads;
+    a.max_seq = kv->max_seq;
+    a.rope_type = c.rope_type;
+    a.in_f32 = in_type == LLMP_IN_F32;
+    a.q8 = kv->q8();
+    a.q8_trunc = kv->dtype == LLMP_KV_Q8_0_TRUNC;
+    a.norm_seq = (c.norm_mode & LLMP_NORM_SEQUENTIAL) != 0;
+    a.v_norm = (c.norm_mode & LLMP_NORM_V) != 0;
+    a.eps = c.eps;
+    LLMP_HIP_CHECK(launch_paged_append(a, D, pick_stream(stream)), "paged append launch");
+    return LLMP_OK;
+}
+
+int llmp_paged_attn(uint64_t handle, int layer, int n_seqs, int n_tokens, int prefix_len, int max_len,
+                    uint64_t seq_start, uint64_t positions, uint64_t blocks, uint64_t q, int64_t q_stride,
+                    uint64_t gate, uint64_t out, int64_t out_stride, uint64_t stream) {
+    if (int rc = ensure_init()) return rc;
+    LLMP_GET_PAGED(kv, handle);
+    if (int rc = paged_layer(kv, layer, "llmp_paged_attn")) return rc;
+    const LayerCfg& c = kv->layers[(size_t)layer];
+    const int D = kv->head_dim;
+    PagedMessage msg;
+    if (int rc = paged_attn_check(kv->paged_shape(), c.n_heads, n_seqs, n_tokens, prefix_len, max_len, seq_start, positions,
+                                  blocks, q, q_stride, gate, out, out_stride, msg))
+        return fail(rc, "%s", msg.text);
+    const PagedPlan p = paged_plan(n_seqs, n_tokens, c.n_heads, kv->n_kv_heads, D, prefix_len,
+                                   max_len > 0 ? max_len : kv->max_seq, G().n_cu);
+    pg::AttnArgs a{};
+    a.pool = kv->paged_planes(layer);
+    a.seq_start = reinterpret_cast<const int*>(seq_start);
+    a.positions = reinterpret_cast<const int*>(positions);
+    a.blocks = reinterpret_cast<const int*>(blocks);
+    a.q = reinterpret_cast<const float*>(q);
+    a.gate = reinterpret_cast<const float*>(gate);
+    a.sinks = c.d_sinks;
+    a.out = reinterpret_cast<float*>(out);
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.width = kv->paged_width();
+    a.n_seqs = n_seqs;
+    a.n_tokens = n_tokens;
+    a.n_heads = c.n_heads;
+    a.group = c.n_heads / kv->n_kv_heads;
+    a.max_seq = kv->max_seq;
+    a.prefix = prefix_len;
+    a.window = layer_window(c);
+    a.prefix_splits = p.prefix_splits;
+    a.own_splits = p.own_splits;
+    a.prefix_tiles = p.prefix_tiles;
+    const float scale = c.scale > 0.0f ? c.scale : (float)(1.0 / std::sqrt((double)D));
+    const float log2e = 1.4426950408889634f;
+    a.qk_scale = c.softcap > 0.0f ? scale : scale * log2e;
+    if (c.softcap > 0.0f) {
+        a.softcap = c.softcap;
+        a.softcap_log2e = c.softcap * log2e;
+        a.inv_softcap = 1.0f / c.softcap;
+    }
+    hipStream_t st = pick_stream(stream);
+    bool capturing;
+    if (int rc = stream_capturing(st, &capturing)) return rc;
+    const size_t rows = (size_t)n_tokens * c.n_heads, splits = (size_t)p.prefix_splits + p.own_splits;
+    const size_t need = rows * splits * (D + 2) * sizeof(float);
+    if (capturing && need > kv->paged_ws.bytes)
+        return fail(LLMP_ERR_INVALID_ARG,
+                    "llmp_paged_attn: a captured call cannot grow its workspace (%zu bytes, %zu held): make it once before",
+                    need, kv->paged_ws.bytes);
+    if (int rc = grow_workspace(kv, kv->paged_ws, need, capturing, st, "paged workspace")) return rc;
+    a.part_o = static_cast<float*>(kv->paged_ws.mem);
+    a.part_ml = a.part_o + rows * splits * D;
+    if (p.prefix_splits > 0)
+        LLMP_HIP_CHECK(launch_paged_attn(a, D, kv->q8(), false, p.prefix_mt, st), "paged attention launch");
+    LLMP_HIP_CHECK(launch_paged_attn(a, D, kv->q8(), true, p.own_mt, st), "paged attention launch");
+    LLMP_HIP_CHECK(launch_paged_combine(a, D, st), "paged combine launch");
     return LLMP_OK;
 }
 

@@ -1,0 +1,245 @@
+// A batch of sequences over one paged KV pool, gfx950: the tables of a step and the append of its
+// tokens.  (The attention over the pool: paged_attn_kernels.h.)
+#pragma once
+
+#include "paged_args.h"
+#include "prefill_kernels.h"
+
+namespace llmp {
+namespace pg {
+
+typedef pk::floatx4 floatx4;
+
+// ---- the tables of a step --------------------------------------------------------------------
+// Per sequence b with len_b rows and grow_b new tokens (grow_b < 0: it has ended), P rows a page:
+//   have = ceil(len/P), need = ceil((len + grow)/P) - have, back = have - shared (ended only);
+//   the returned blocks [shared, have) of the ended sequences are pushed on the free stack in
+//   order of (b, block), then the blocks [have, have + need) of the others are popped from its top
+//   in the same order; seq_start is the exclusive sum of the new tokens, and token i of sequence b
+//   has position len_b + i and slot blocks[b][pos / P] * P + pos % P.
+constexpr int kTablesThreads = 1024;
+inline size_t tables_lds(int n) { return ((size_t)n * 4 + 3) * sizeof(int); }
+
+// Every workgroup reads all lengths and forms the three exclusive sums itself (a few KB out of
+// L2), then takes its share of the tokens, blocks and returned pages: one launch, no exchange.
+// len_out and n_free_out may lie over the inputs, so the workgroup that is last to have read them
+// writes both.  Bound by latency: three dependent memory trips and the scan's barriers.
+__global__ __launch_bounds__(kTablesThreads) void paged_tables_kernel(TablesArgs a) {
+    extern __shared__ int s_dyn[];
+    const int n = a.n, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int* s_len = s_dyn;              // n: the length, or ~length for a sequence that has ended
+    int* s_start = s_len + n;        // n + 1
+    int* s_need = s_start + n + 1;   // n + 1
+    int* s_back = s_need + n + 1;    // n + 1
+    __shared__ long long s_sum[3][kTablesThreads / 64];
+    __shared__ int s_last;
+    const int n_free = *a.n_free;
+    const int P1 = (1 << a.shift) - 1;
+    int bad = n_free < 0 || n_free > a.n_pages;
+    for (int i = tid; i < n; i += kTablesThreads) {
+        const int l = a.len[i], g = a.grow[i];
+        const bool ended = g < 0;
+        const int add = ended ? 0 : g;
+        const bool wrong = l < 0 || (long long)l + add > a.max_seq;
+        bad |= wrong;
+        const int len = wrong ? 0 : l, grow = wrong ? 0 : add;
+        const int have = (int)(((unsigned)len + P1) >> a.shift);
+        const int after = (int)(((unsigned)len + (unsigned)grow + P1) >> a.shift);
+        s_len[i] = ended ? ~len : len;
+        s_start[i] = grow;
+        s_need[i] = ended ? 0 : after - have;
+        s_back[i] = ended && !wrong ? max(have - a.shared, 0) : 0;
+    }
+    bad = __syncthreads_or(bad);
+    // Exclusive sums: each thread over its `per` consecutive sequences, the wave by shuffles, the
+    // waves through LDS.
+    const int per = (n + kTablesThreads - 1) / kTablesThreads;
+    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    long long own[3] = {0, 0, 0};
+    for (int i = i0; i < i1; ++i) {
+        own[0] += s_start[i];
+        own[1] += s_need[i];
+        own[2] += s_back[i];
+    }
+    long long at[3];
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        long long x = own[q];
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const long long y = __shfl_up(x, off);
+            if (lane >= off) x += y;
+        }
+        if (lane == 63) s_sum[q][wave] = x;
+        at[q] = x - own[q];
+    }
+    __syncthreads();
+    long long total[3] = {0, 0, 0};
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+        for (int w = 0; w < kTablesThreads / 64; ++w) {
+            if (w == wave) at[q] += total[q];
+            total[q] += s_sum[q][w];
+        }
+    int status = 0;
+    if (bad || n_free + total[2] > a.n_pages) status = -1;
+    else if (total[0] > a.max_tokens) status = -2;
+    else if (total[1] > n_free + total[2]) status = (int)min(total[1] - n_free - total[2], (long long)0x7fffffff);
+    const bool good = status == 0;
+    for (int i = i0; i < i1; ++i) {   // the thread's own entries: no other thread reads them yet
+        const int x = s_start[i], y = s_need[i], z = s_back[i];
+        s_start[i] = good ? (int)at[0] : 0;
+        s_need[i] = good ? (int)at[1] : 0;
+        s_back[i] = good ? (int)at[2] : 0;
+        at[0] += x;
+        at[1] += y;
+        at[2] += z;
+    }
+    const int tokens = good ? (int)total[0] : 0, need = good ? (int)total[1] : 0, back = good ? (int)total[2] : 0;
+    if (tid == 0) {
+        s_start[n] = tokens;
+        s_need[n] = need;
+        s_back[n] = back;
+        s_last = 1;
+        // All inputs of this workgroup are in LDS and registers (the barriers above): the last
+        // workgroup to come here may write over them.
+        if (gridDim.x > 1) {
+            __threadfence();
+            const int t = atomicAdd(a.ticket, 1);
+            s_last = t == (int)gridDim.x - 1;
+            if (s_last) *a.ticket = 0;
+        }
+    }
+    __syncthreads();
+    // Entry e of the stack after the pushes, as the popping tokens see it.
+    const int top = n_free + back;
+    auto returned = [&](int r) {
+        const int b = paged_owner(s_back, n, r);
+        return a.blocks[(long long)b * a.width + a.shared + (r - s_back[b])];
+    };
+    auto popped = [&](int rank) {
+        const int e = top - 1 - rank;
+        return e < n_free ? a.free_pages[e] : returned(e - n_free);
+    };
+    const int g0 = blockIdx.x * kTablesThreads + tid, gn = gridDim.x * kTablesThreads;
+    for (int i = g0; i <= n; i += gn) a.seq_start[i] = s_start[i];
+    for (int i = g0; i < a.max_tokens; i += gn) {
+        int pos = -1, slot = -1;
+        if (i < tokens) {
+            const int b = paged_owner(s_start, n, i);
+            const int len = s_len[b];   // not an ended one: those hold no tokens
+            pos = len + (i - s_start[b]);
+            const int j = pos >> a.shift, have = (int)(((unsigned)len + P1) >> a.shift);
+            const int page = j < have ? a.blocks[(long long)b * a.width + j] : popped(s_need[b] + j - have);
+            if (paged_page_ok(page, a.n_pages)) slot = (page << a.shift) + (pos & P1);
+        }
+        a.positions[i] = pos;
+        a.slots[i] = slot;
+    }
+    for (int r = g0; r < need; r += gn) {
+        const int b = paged_owner(s_need, n, r);
+        const int have = (int)(((unsigned)s_len[b] + P1) >> a.shift);
+        a.blocks[(long long)b * a.width + have + (r - s_need[b])] = popped(r);
+    }
+    for (int r = g0; r < back; r += gn) a.free_pages[n_free + r] = returned(r);
+    if (blockIdx.x == 0 && tid == 0) *a.status = status;
+    if (s_last) {
+        for (int i = tid; i < n; i += kTablesThreads) {
+            const int l = s_len[i];
+            const bool ended = l < 0;
+            // (a refused step leaves every length as it was, a wrong one included)
+            if (good) a.len_out[i] = ended ? 0 : l + (s_start[i + 1] - s_start[i]);
+            else if (a.len_out != a.len) a.len_out[i] = a.len[i];
+        }
+        if (tid == 0) *a.n_free_out = good ? top - need : n_free;
+    }
+}
+
+// ---- rotation and append ---------------------------------------------------------------------
+constexpr int kAppendThreads = 256;
+
+__device__ __forceinline__ floatx4 load4_in(const void* p, long long i, int f32) {
+    if (f32) return *reinterpret_cast<const floatx4*>(static_cast<const float*>(p) + i);
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(p) + i);
+    return floatx4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u),
+                   __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u)};
+}
+
+// One workgroup = (token, group of kAppendHeads heads): the heads [h0, h0 + kAppendHeads) of the token's
+// query, key and value heads in that order, staged in LDS and prepared with the decode path's
+// functions, so the stored rows are bit-identical to a decode append's.
+constexpr int kAppendHeads = 8;
+template <int D>
+__global__ __launch_bounds__(kAppendThreads) void paged_append_lds_kernel(AppendArgs a) {
+    __shared__ float s_x[kAppendHeads * D], s_acc[kAppendHeads * 8], s_r[kAppendHeads], s_inv[kAppendHeads * (D / 32)];
+    const int tid = threadIdx.x, t = blockIdx.x;
+    const int Hq = a.n_heads, Hkv = a.pool.n_kv_heads;
+    const int pos = a.positions[t], slot = a.k != nullptr ? a.slots[t] : -1;   // (slots may be null without k)
+    if ((unsigned)pos >= (unsigned)a.max_seq) return;
+    const bool store = a.k != nullptr && paged_slot_ok(slot, a.pool.shift, a.pool.n_pages);
+    const int all = a.k != nullptr ? Hq + 2 * Hkv : Hq;
+    const int h0 = blockIdx.y * kAppendHeads, h1 = min(h0 + kAppendHeads, all), nh = h1 - h0;
+    if (!store && h0 >= Hq) return;
+    for (int e = tid; e < nh * D; e += kAppendThreads) {
+        const int hh = h0 + e / D, d = e % D;
+        const bool is_q = hh < Hq, is_k = hh < Hq + Hkv;
+        const void* p = is_q ? a.q : is_k ? a.k : a.v;
+        const long long row = is_q ? a.q_stride * t + (long long)hh * D
+                              : is_k ? a.k_stride * t + (long long)(hh - Hq) * D
+                                     : a.v_stride * t + (long long)(hh - Hq - Hkv) * D;
+        s_x[e] = pk::in_val(p, row + d, a.in_f32);
+    }
+    __syncthreads();
+    const long long row = (long long)pos * a.half_rope;
+    const dk::HeadPrep hp{a.qnw, a.knw, a.eps, a.cos_t ? a.cos_t + row : nullptr, a.sin_t ? a.sin_t + row : nullptr,
+                          a.half_rope, a.rope_type};
+    const int nq = max(min(h1, Hq) - h0, 0), nk = max(min(h1, Hq + Hkv) - h0 - nq, 0);
+    if (a.norm_seq) {   // the sequential order is the key norm's only
+        if (nq) dk::prep_heads_lds<D, kAppendThreads>(s_x, nq, nq, s_acc, s_r, hp, tid);
+        if (nk) dk::prep_heads_lds<D, kAppendThreads>(s_x + nq * D, nk, 0, s_acc, s_r, hp, tid, true);
+    } else if (nq + nk) {
+        dk::prep_heads_lds<D, kAppendThreads>(s_x, nq + nk, nq, s_acc, s_r, hp, tid);
+    }
+    const int nv = nh - nq - nk;
+    if (a.v_norm && nv) {
+        float* sv = s_x + (nq + nk) * D;
+        if (tid < nv) s_r[tid] = dk::seq_rms_inv<D>(sv + tid * D, a.eps);
+        __syncthreads();
+        for (int e = tid; e < nv * D; e += kAppendThreads) sv[e] = sv[e] * s_r[e / D];
+    }
+    __syncthreads();
+    for (int e = tid; e < nq * D; e += kAppendThreads) a.out[a.out_stride * t + (long long)h0 * D + e] = s_x[e];
+    if (!store || nk + nv == 0) return;
+    const int page = slot >> a.pool.shift, r = slot & ((1 << a.pool.shift) - 1);
+    auto row_of = [&](int hh) {   // row index of head hh (>= Hq) in its plane
+        const int h = (hh - Hq) % Hkv;
+        return (((long long)page * Hkv + h) << a.pool.shift) + r;
+    };
+    if (!a.q8) {
+        for (int e = tid + nq * D; e < nh * D; e += kAppendThreads) {
+            const int hh = h0 + e / D;
+            static_cast<float*>(hh < Hq + Hkv ? a.pool.k : a.pool.v)[row_of(hh) * D + e % D] = s_x[e];
+        }
+        return;
+    }
+    constexpr int NB = D / 32;
+    for (int b = tid + nq * NB; b < nh * NB; b += kAppendThreads) {
+        const int hh = h0 + b / NB;
+        const float scale = dk::q8_block_scale(s_x + 32 * b);
+        s_inv[b] = dk::q8_inv_scale(scale);
+        (hh < Hq + Hkv ? a.pool.ks : a.pool.vs)[row_of(hh) * NB + b % NB] = scale;
+    }
+    __syncthreads();
+    for (int w = tid + nq * D / 4; w < nh * D / 4; w += kAppendThreads) {
+        const int e = 4 * w, hh = h0 + e / D;
+        unsigned word = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            word |= (unsigned)(dk::q8_code(s_x[e + j], s_inv[e / 32], a.q8_trunc != 0) & 0xFF) << (8 * j);
+        *reinterpret_cast<unsigned*>(static_cast<signed char*>(hh < Hq + Hkv ? a.pool.k : a.pool.v) + row_of(hh) * D +
+                                     e % D) = word;
+    }
+}
+
+}  // namespace pg
+}  // namespace llmp

@@ -344,24 +344,12 @@ def kernel_group(head_size: int, group: int) -> int:
     return 0
 
 
-class HipForwardPass:
-    """Attention section of a GPU-resident forward pass on MI355X.
+class LayerSetup:
+    """The set-up of a handle's RoPE tables and layers from a ModelConfig, for the classes that own a
+    handle (self.kv.handle) with self.config and self.max_seq_len."""
 
-    Mirrors the CudaForwardPass constructor's attention set-up (CudaForwardPass.java:346-416:
-    RoPE table upload, per-layer zero-filled KV, QK-norm weights) and its attention API.
-    `qk_norm` holds per-layer (q_weights, k_weights) arrays of head_size floats, or None."""
-
-    def __init__(self, config: ModelConfig, max_seq_len: int,
-                 qk_norm: Optional[Sequence[Optional[tuple]]] = None, device: int = 0,
-                 kv_dtype: int = _lib.LLMP_KV_F32,
-                 sinks: Optional[Sequence[Optional[np.ndarray]]] = None):
-        if not HipForwardPass.isSupportedForAttention(config):
-            raise LlmpError("HipForwardPass", 6, "configuration not supported by the HIP attention path")
-        init(device)
-        self.config = config
-        self.max_seq_len = max_seq_len
-        c = config
-        self.kv = KvCache(c.block_count, max_seq_len, c.head_count_kv, c.head_size, kv_dtype)
+    def _upload_rope(self) -> None:
+        c, max_seq_len = self.config, self.max_seq_len
         rope_dim = c.rope_dim_count or c.head_size
         # InferenceEngine.java:58-78: global table with linear scaling; local table for
         # Gemma 3 (theta 10000) and Gemma 4 (SWA theta) when a sliding window exists.  The MoE
@@ -384,40 +372,7 @@ class HipForwardPass:
             call("llmp_rope_upload", self.kv.handle, _lib.LLMP_ROPE_SEL_LOCAL, _fp(cos_l),
                  _fp(sin_l), max_seq_len, rope_dim // 2)
             self.has_local_rope = True
-        for layer in range(c.block_count):
-            w = qk_norm[layer] if qk_norm is not None else None
-            self.configure_layer(layer, w)
-            if sinks is not None and sinks[layer] is not None:
-                self.set_sinks(layer, sinks[layer])
-        self.gpuQ = DeviceBuffer(c.q_dim * 4)
-        self.gpuK = DeviceBuffer(c.kv_dim * 4)
-        self.gpuV = DeviceBuffer(c.kv_dim * 4)
-        self.gpuXb2 = DeviceBuffer(c.q_dim * 4)
-        self.gpuGate = DeviceBuffer(c.q_dim * 4)   # attention output gate (Qwen3.5)
-        # [position, position + 1] as int32 (CudaForwardPass.gpuTokenParams, :138-141)
-        self.gpuTokenParams = DeviceBuffer(8)
 
-    # -- reflection-contract statics -------------------------------------------------------
-    @staticmethod
-    def isSupportedForAttention(config: ModelConfig, weights=None) -> bool:
-        """CudaForwardPass.isSupportedForAttention (CudaForwardPass.java:1223-1244) rejects
-        LayerNorm models; the HIP section also needs a head shape it has a kernel for."""
-        if config.use_layer_norm:
-            return False
-        if config.head_count <= 0 or config.head_count_kv <= 0:
-            return False
-        if config.head_count % config.head_count_kv:
-            return False
-        group = config.head_count // config.head_count_kv
-        if kernel_group(config.head_size, group) == 0:
-            return False
-        rd = config.rope_dim_count or config.head_size
-        return rd % 2 == 0 and rd <= config.head_size
-
-    def getGpuLayerCount(self) -> int:
-        return self.config.block_count
-
-    # -- set-up ------------------------------------------------------------------------------
     def configure_layer(self, layer: int, qk_norm: Optional[tuple]) -> None:
         c = self.config
         is_global = is_global_layer(c.architecture, layer, c.sliding_window_pattern, c.expert_count)
@@ -453,6 +408,59 @@ class HipForwardPass:
         if s.size != self.config.head_count:
             raise ValueError(f"sinks: {s.size} values for {self.config.head_count} heads")
         call("llmp_layer_sinks", self.kv.handle, layer, _fp(s))
+
+
+class HipForwardPass(LayerSetup):
+    """Attention section of a GPU-resident forward pass on MI355X.
+
+    Mirrors the CudaForwardPass constructor's attention set-up (CudaForwardPass.java:346-416:
+    RoPE table upload, per-layer zero-filled KV, QK-norm weights) and its attention API.
+    `qk_norm` holds per-layer (q_weights, k_weights) arrays of head_size floats, or None."""
+
+    def __init__(self, config: ModelConfig, max_seq_len: int,
+                 qk_norm: Optional[Sequence[Optional[tuple]]] = None, device: int = 0,
+                 kv_dtype: int = _lib.LLMP_KV_F32,
+                 sinks: Optional[Sequence[Optional[np.ndarray]]] = None):
+        if not HipForwardPass.isSupportedForAttention(config):
+            raise LlmpError("HipForwardPass", 6, "configuration not supported by the HIP attention path")
+        init(device)
+        self.config = config
+        self.max_seq_len = max_seq_len
+        c = config
+        self.kv = KvCache(c.block_count, max_seq_len, c.head_count_kv, c.head_size, kv_dtype)
+        self._upload_rope()
+        for layer in range(c.block_count):
+            w = qk_norm[layer] if qk_norm is not None else None
+            self.configure_layer(layer, w)
+            if sinks is not None and sinks[layer] is not None:
+                self.set_sinks(layer, sinks[layer])
+        self.gpuQ = DeviceBuffer(c.q_dim * 4)
+        self.gpuK = DeviceBuffer(c.kv_dim * 4)
+        self.gpuV = DeviceBuffer(c.kv_dim * 4)
+        self.gpuXb2 = DeviceBuffer(c.q_dim * 4)
+        self.gpuGate = DeviceBuffer(c.q_dim * 4)   # attention output gate (Qwen3.5)
+        # [position, position + 1] as int32 (CudaForwardPass.gpuTokenParams, :138-141)
+        self.gpuTokenParams = DeviceBuffer(8)
+
+    # -- reflection-contract statics -------------------------------------------------------
+    @staticmethod
+    def isSupportedForAttention(config: ModelConfig, weights=None) -> bool:
+        """CudaForwardPass.isSupportedForAttention (CudaForwardPass.java:1223-1244) rejects
+        LayerNorm models; the HIP section also needs a head shape it has a kernel for."""
+        if config.use_layer_norm:
+            return False
+        if config.head_count <= 0 or config.head_count_kv <= 0:
+            return False
+        if config.head_count % config.head_count_kv:
+            return False
+        group = config.head_count // config.head_count_kv
+        if kernel_group(config.head_size, group) == 0:
+            return False
+        rd = config.rope_dim_count or config.head_size
+        return rd % 2 == 0 and rd <= config.head_size
+
+    def getGpuLayerCount(self) -> int:
+        return self.config.block_count
 
     # -- per-token API -------------------------------------------------------------------------
     def uploadQKV(self, q: np.ndarray, k: np.ndarray, v: np.ndarray) -> None:
