@@ -165,9 +165,18 @@ __device__ __forceinline__ floatx4 load4_in(const void* p, long long i, int f32)
                    __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u)};
 }
 
+// Scale of 32 values: their largest magnitude times 1/127, in one product (a contiguous cache divides;
+// the two differ by at most one unit in the last place).
+constexpr float kInv127 = 1.0f / 127.0f;
+__device__ __forceinline__ float block_scale(const float* x) {
+    float mx = 0.0f;
+    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fabsf(x[i]));
+    return mx * kInv127;
+}
+
 // One workgroup = (token, group of kAppendHeads heads): the heads [h0, h0 + kAppendHeads) of the token's
 // query, key and value heads in that order, staged in LDS and prepared with the decode path's
-// functions, so the stored rows are bit-identical to a decode append's.
+// functions, so the rows are bit-identical to a decode append's (before they are quantised).
 constexpr int kAppendHeads = 8;
 template <int D>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_lds_kernel(AppendArgs a) {
@@ -225,7 +234,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_lds_kernel(Append
     constexpr int NB = D / 32;
     for (int b = tid + nq * NB; b < nh * NB; b += kAppendThreads) {
         const int hh = h0 + b / NB;
-        const float scale = dk::q8_block_scale(s_x + 32 * b);
+        const float scale = block_scale(s_x + 32 * b);
         s_inv[b] = dk::q8_inv_scale(scale);
         (hh < Hq + Hkv ? a.pool.ks : a.pool.vs)[row_of(hh) * NB + b % NB] = scale;
     }

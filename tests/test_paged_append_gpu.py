@@ -1,5 +1,6 @@
 """GPU checks of llmp_paged_append: queries against the rotation in 64 bits, stored rows bit for bit
-against a contiguous cache's decode appends, and what must stay untouched."""
+against a contiguous cache's decode appends (quantised on the host for Q8_0 pools), and what must stay
+untouched."""
 import ctypes as C
 
 import numpy as np
@@ -86,7 +87,7 @@ def test_append(hq, hkv, D, page, T, rope_type, rope_dim, norm, norm_mode, cache
     slots = rng.permutation(n_pages * page)[:T].astype(I)
     with pc.Device() as d:
         kv = PagedKv(1, n_pages, page, MAX_SEQ, hkv, D, cache)
-        ref = hfp.KvCache(1, MAX_SEQ, hkv, D, cache) if D != 96 or cache == 0 else None
+        ref = hfp.KvCache(1, MAX_SEQ, hkv, D)
         try:
             for h in (kv.handle, ref.handle):
                 config(h, hq, hkv, D, rope_type, rope_dim, qw, kw, norm_mode, tables)
@@ -128,9 +129,15 @@ def test_append(hq, hkv, D, page, T, rope_type, rope_dim, norm, norm_mode, cache
                 if cache == 0:
                     k, v = ref.read(0, int(positions[t]), 1)
                     rk = {"k": k, "v": v}
-                else:
-                    a = ref.read_q8(0, int(positions[t]), 1)
-                    rk = dict(zip(("k", "ks", "v", "vs"), a))
+                else:   # the fp32 rows of a fp32 cache, quantised
+                    rk = dict(zip(("k", "v"), ref.read(0, int(positions[t]), 1)))
+                    for w in "kv":
+                        x = rk[w].reshape(-1, 32)
+                        rk[w + "s"] = np.abs(x).max(1) * F32(1 / 127)
+                        with np.errstate(divide="ignore"):
+                            y = x * np.where(rk[w + "s"] > 0, F32(1) / rk[w + "s"], F32(0))[:, None]
+                        y = np.trunc(y) if cache == 2 else np.floor(y) + (y - np.floor(y) >= F32(0.5))
+                        rk[w] = np.clip(y, -128, 127).astype(np.int8)
                 for w, x in rk.items():
                     mine = held[w][pg, :, r]
                     assert np.array_equal(mine.reshape(-1).view(np.uint8), np.ascontiguousarray(x).reshape(-1).view(np.uint8)), (t, w)
