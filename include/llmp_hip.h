@@ -476,9 +476,9 @@ int llmp_paged_tables(uint64_t handle, int n_seqs, int shared_blocks, int max_to
  * with the layer's table (llmp_rope_upload: interleaved or half layout, part of the head, linear or
  * YaRN scaling are all the table's and llmp_layer_config's), and written to q_out as fp32; its K row is
  * treated likewise and stored with its V row at slots[t], in a contiguous cache's decode arithmetic:
- * fp32 rows equal llmp_attn_decode's bit for bit.  Q8_0 pools hold them quantised: block scale
- * max|x| * (1/127) (a product where a contiguous cache divides, one unit in the last place at most),
- * quants x * (1/scale) rounded half up or truncated by the handle's dtype, as there.
+ * fp32 and LLMP_KV_Q8_0_TRUNC rows equal llmp_attn_decode's bit for bit; LLMP_KV_Q8_0 rows are
+ * rounded as there, with block scales max|x| * (1/127) (a product where a contiguous cache divides:
+ * one unit in the last place at most).
  * k = v = 0: only the queries (slots may be 0).  in_type: the type of q, k and v (LLMP_IN_*); strides
  * in elements, at least a row; q_out may be q for fp32 at equal strides.  A token with no position is
  * skipped, its q_out row too.  No two tokens may name one slot. */

@@ -113,12 +113,11 @@ struct AppendArgs;
 struct AttnArgs;
 }
 // A batch of sequences over a paged pool (paged_kernels.h, paged_attn_kernels.h): the tables of a
-// step, the append of its tokens, and its attention: partials of the prefix rows (own = false) or of
-// each sequence's own rows with 16*mt query rows a workgroup (mt 1, 2, and 4 up to head_dim 128),
-// joined by the combine.
+// step, the append of its tokens, and its attention: partials of the prefix rows and of each sequence's
+// own rows in one launch, with items of the sizes that paged_plan gives, joined by the combine.
 hipError_t launch_paged_tables(const pg::TablesArgs& a, hipStream_t stream);
 hipError_t launch_paged_append(const pg::AppendArgs& a, int head_dim, hipStream_t stream);
-hipError_t launch_paged_attn(const pg::AttnArgs& a, int head_dim, bool q8, bool own, int mt, hipStream_t stream);
+hipError_t launch_paged_attn(const pg::AttnArgs& a, int head_dim, bool q8, int prefix_wide, int own_wide, hipStream_t stream);
 hipError_t launch_paged_combine(const pg::AttnArgs& a, int head_dim, hipStream_t stream);
 
 // Plain 16-byte-per-thread copy kernel.

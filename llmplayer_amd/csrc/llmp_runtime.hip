@@ -2222,9 +2222,7 @@ int llmp_paged_attn(uint64_t handle, int layer, int n_seqs, int n_tokens, int pr
     if (int rc = grow_workspace(kv, kv->paged_ws, need, capturing, st, "paged workspace")) return rc;
     a.part_o = static_cast<float*>(kv->paged_ws.mem);
     a.part_ml = a.part_o + rows * splits * D;
-    if (p.prefix_splits > 0)
-        LLMP_HIP_CHECK(launch_paged_attn(a, D, kv->q8(), false, p.prefix_mt, st), "paged attention launch");
-    LLMP_HIP_CHECK(launch_paged_attn(a, D, kv->q8(), true, p.own_mt, st), "paged attention launch");
+    LLMP_HIP_CHECK(launch_paged_attn(a, D, kv->q8(), p.prefix_wide, p.own_wide, st), "paged attention launch");
     LLMP_HIP_CHECK(launch_paged_combine(a, D, st), "paged combine launch");
     return LLMP_OK;
 }

@@ -1,5 +1,5 @@
-// Launches of the paged batch's tables, append and combine (paged_kernels.h), and the choice of the
-// attention kernel.
+// Launches of the paged batch's tables and append (paged_kernels.h) and of the attention's combine
+// (paged_attn_kernels.h).
 #include "paged_attn_kernels.h"
 #include "paged_kernels.h"
 
@@ -24,9 +24,9 @@ hipError_t launch_append_d(const pg::AppendArgs& a, hipStream_t st) {
 
 template <int D>
 hipError_t launch_combine_d(const pg::AttnArgs& a, hipStream_t st) {
-    constexpr int RPB = pg::kJoinThreads / (D / 4);
+    const int per = pg::join_groups<D>() / pg::join_groups_per_row<D>(a.prefix_splits + a.own_splits);
     const long long rows = (long long)a.n_tokens * a.n_heads;
-    hipLaunchKernelGGL((pg::paged_combine_kernel<D>), dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(pg::kJoinThreads), 0, st, a);
+    hipLaunchKernelGGL((pg::paged_combine_kernel<D>), dim3((unsigned)((rows + per - 1) / per)), dim3(pg::kJoinThreads), 0, st, a);
     return hipGetLastError();
 }
 

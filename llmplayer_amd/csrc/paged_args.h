@@ -66,6 +66,8 @@ struct AttnArgs {
     int prefix, window;
     int prefix_splits, own_splits;   // partials of a row: the prefix's, then its own rows'
     int prefix_tiles;                // 32-row tiles of one prefix split
+    int prefix_items, own_items;     // blocks of query rows per (KV head, split)
+    int prefix_wgs;                  // workgroups of the prefix items, padded to a multiple of 8
     float qk_scale, softcap, softcap_log2e, inv_softcap;
 };
 

@@ -9,15 +9,19 @@
 // tokens.  Every item leaves (m, l = sum 2^(s - m), unnormalised o) per query row, and
 // paged_combine_kernel joins the items of a row.
 //
-// One wave takes 32 rows of the pool at a time against all MT tiles of 16 query rows, straight from
-// memory to registers: S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_16x16x32_f16.  Lane
-// (n = lane % 16, g = lane / 16) holds A[n][8g + j], B[8g + j][n] and D[4g + i][n]:
+// 32 rows of the pool are taken at a time, S^T = K Q^T and O^T += V^T P^T with
+// v_mfma_f32_16x16x32_f16.  Lane (n = lane % 16, g = lane / 16) holds A[n][8g + j], B[8g + j][n] and
+// D[4g + i][n]:
 //  - K: lane (n, g) loads dims 32s + 8g .. +7 of rows n and 16 + n: the A operands as they are.
 //  - S^T's result lies as (query n, rows 4g + i), which is the B operand of the second product when
 //    its 32 rows are taken in the order {4g .. 4g+3, 16 + 4g .. 16 + 4g + 3}.
 //  - V: lane (n, g) loads dims 64c + 4n .. +3 of those 8 rows, 256 contiguous bytes a row.  Column t
 //    of the four is one A operand whose 16 output rows stand for dims 64c + 4n + t: the transposition
 //    costs nothing.
+// Few query rows (attn_narrow, 16): each wave takes tiles of its own, straight from memory to registers
+// to the matrix units, and the waves join at the end.  Many (attn_wide, 64 or 128): the four waves share
+// each tile, every wave loads and splits a quarter of it into LDS, laid out as the operands are read, and
+// multiplies all of it with query rows of its own.
 // Precision: each fp32 operand is split in two fp16 parts and a product takes three MFMAs
 // (hi*hi + hi*lo + lo*hi, ~2^-21 per term).  fp16 reaches from 2^-24 to 65504, so K is scaled by a
 // power of two per 32 rows, V by one per wave that only grows, each query by its own: the parts
@@ -110,7 +114,9 @@ struct Tile<D, false> {
     static __device__ __forceinline__ float clean(float x, unsigned keep, unsigned& worst) {
         const unsigned b = __float_as_uint(x) & keep, m = b & 0x7FFFFFFFu;
         worst = max(worst, m);
-        return __uint_as_float(b & (unsigned)((int)(m - 0x7F800000u) >> 31));   // no lane mask per value
+        int fin = (int)(m - 0x7F800000u) >> 31;   // all ones where it is finite
+        asm("" : "+v"(fin));                      // (not a lane mask per value: they would not fit)
+        return __uint_as_float(b & (unsigned)fin);
     }
     // ok: bit u of the lane's K rows; returns bit u for a K row with a value that is not finite.
     __device__ __forceinline__ unsigned clean_k(unsigned ok) {
@@ -283,19 +289,22 @@ __device__ __forceinline__ int fit_exp(float mx) {
     return mx == 0.0f ? 0 : max(min(b, 120), -120);
 }
 
-// The rows of a tile (bit = row) that the lanes' bits name: bk the K rows n and 16 + n, bv the V
-// rows 4g + i and 16 + 4g + i.
-__device__ __forceinline__ unsigned tile_rows(unsigned bk, unsigned bv, int n, int g) {
-    unsigned x = (bk & 1u) << n | (bk >> 1) << (16 + n) | (bv & 15u) << (4 * g) | (bv >> 4) << (16 + 4 * g);
+__device__ __forceinline__ unsigned wave_or(unsigned x) {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) x |= __shfl_xor(x, off);
     return __builtin_amdgcn_readfirstlane(x);
 }
 
-template <int D, int MT>
-constexpr size_t attn_lds() {
-    const size_t q = (size_t)MT * (D / 32) * 2 * 64 * 16, x = 2 * (size_t)MT * (D / 4 + 2) * 64 * 4;
-    return q > x ? q : x;
+// The rows of a tile (bit = row) that the lanes' bits name: bk the K rows n and 16 + n, bv the V
+// rows 4g + i and 16 + 4g + i.
+__device__ __forceinline__ unsigned tile_rows(unsigned bk, unsigned bv, int n, int g) {
+    return wave_or((bk & 1u) << n | (bk >> 1) << (16 + n) | (bv & 15u) << (4 * g) | (bv >> 4) << (16 + 4 * g));
+}
+
+// Dynamic LDS: the waves' states that attn_narrow joins, or attn_wide's tile.
+template <int D>
+constexpr size_t attn_lds(int wide) {
+    return wide ? (size_t)(D / 16 + D / 16) * 2 * 64 * 16 : 2 * (size_t)(D / 4 + 2) * 64 * 4;
 }
 
 // The sequence of work item `item` of an own-rows launch (paged_item_base).
@@ -311,159 +320,241 @@ __device__ __forceinline__ int item_sequence(const AttnArgs& a, int item, int BM
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// OWN: blockIdx = (item of item_sequence, KV head, split of the own rows).
-// Else: blockIdx = (block of 16*MT query rows of all tokens, KV head, split of the prefix).
-template <int D, int MT, bool Q8, bool OWN>
-__global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(AttnArgs a) {
-    using T = Tile<D, Q8>;
-    constexpr int KS = D / 32, DT = D / 16, BM = 16 * MT, NC = D / 64, REM = D % 64 / 32;
-    extern __shared__ uint4 s_dyn4[];
-    __shared__ int s_pos[BM], s_first[BM];
-    __shared__ float s_fq[BM];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-    const int h = blockIdx.y, split = blockIdx.z;
-    const int G = a.group;
-    // Query rows of the item: token tok0 + r / G, head h*G + r % G for r in [r0, r1).
-    int tok0 = 0, r0, r1;
-    const int* blk = a.blocks;
+// The query rows of a work item: `rows` per item of one KV head, of all tokens (prefix) or of one
+// sequence (OWN).
+struct ItemRows {
+    int tok0, r0, r1;     // token tok0 + r / G, head h*G + r % G for r in [r0, r1)
+    const int* blk;       // the block table
+};
+template <bool OWN>
+__device__ __forceinline__ ItemRows item_rows(const AttnArgs& a, int item, int rows, int lane) {
+    ItemRows x{0, item * rows, 0, a.blocks};
     if constexpr (OWN) {
-        const int b = item_sequence(a, blockIdx.x, BM, lane);
+        const int b = item_sequence(a, item, rows, lane);
         const int st = min(max(a.seq_start[b], 0), a.n_tokens), en = min(max(a.seq_start[b + 1], st), a.n_tokens);
-        tok0 = st;
-        r0 = ((int)blockIdx.x - paged_item_base(st, G, BM, b)) * BM;
-        r1 = min((en - st) * G, r0 + BM);
-        if (r0 < 0) return;
-        blk += (long long)b * a.width;
+        x.tok0 = st;
+        x.r0 = (item - paged_item_base(st, a.group, rows, b)) * rows;
+        x.r1 = x.r0 < 0 ? x.r0 : min((en - st) * a.group, x.r0 + rows);
+        x.blk += (long long)b * a.width;
     } else {
-        r0 = blockIdx.x * BM;
-        r1 = min(min(max(a.seq_start[a.n_seqs], 0), a.n_tokens) * G, r0 + BM);
+        x.r1 = min(min(max(a.seq_start[a.n_seqs], 0), a.n_tokens) * a.group, x.r0 + rows);
     }
-    if (r0 >= r1) return;
+    return x;
+}
 
-    // Queries: wave w prepares the tiles w, w + 4, ...: scaled, divided by a power of two of their
-    // own, split and laid out as the B operands take them.
-    uint4* s_q = s_dyn4;
-    for (int mt = wave; mt < MT; mt += kAttnWaves) {
-        const int r = r0 + 16 * mt + n;
-        const bool have = r < r1;
-        const int rr = have ? r : r0, tok = tok0 + rr / G, head = h * G + rr % G;
-        const float* q = a.q + (long long)tok * a.q_stride + (long long)head * D + 8 * g;
-        int pos = a.positions[tok];
-        float x[KS][8], mx = 0.0f;
+// One tile of 16 query rows: scaled, divided by a power of two of their own (returned as fq), split, as
+// the B operands take them; pos and first: the rows of the sequence that the lane's query attends.
+template <int D>
+__device__ __forceinline__ void load_queries(const AttnArgs& a, const ItemRows& x, int r, int h, int g, f16x8 (&qh)[D / 32],
+                                             f16x8 (&ql)[D / 32], float& fq, int& pos, int& first) {
+    constexpr int KS = D / 32;
+    const bool have = r < x.r1;
+    const int rr = have ? r : x.r0, tok = x.tok0 + rr / a.group, head = h * a.group + rr % a.group;
+    const float* q = a.q + (long long)tok * a.q_stride + (long long)head * D + 8 * g;
+    const int p = a.positions[tok];
+    float v[KS][8], mx = 0.0f;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) pk::load8(q + 32 * s, x[s]);
+    for (int s = 0; s < KS; ++s) pk::load8(q + 32 * s, v[s]);
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[s][e] *= a.qk_scale;
-                mx = fmaxf(mx, fabsf(x[s][e]));
-            }
-        mx = dk::lane_step<16, true>(mx);
-        mx = dk::lane_step<32, true>(mx);
-        const int e = finite_bits(__float_as_uint(mx)) ? fit_exp(mx) : 0;
-        const float f = pk::pow2i(-e);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[s][i] *= f;
-            f16x8 hi, lo;
-            split8(x[s], hi, lo);
-            s_q[((mt * KS + s) * 2 + 0) * 64 + lane] = __builtin_bit_cast(uint4, hi);
-            s_q[((mt * KS + s) * 2 + 1) * 64 + lane] = __builtin_bit_cast(uint4, lo);
+        for (int e = 0; e < 8; ++e) {
+            v[s][e] *= a.qk_scale;
+            mx = fmaxf(mx, fabsf(v[s][e]));
         }
-        if (g == 0) {
-            const bool live = have && (unsigned)pos < (unsigned)a.max_seq;
-            s_pos[16 * mt + n] = live ? pos : -1;
-            s_first[16 * mt + n] = !live ? 0x7fffffff : a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
-            s_fq[16 * mt + n] = pk::pow2i(e);
-        }
+    mx = dk::lane_step<16, true>(mx);
+    mx = dk::lane_step<32, true>(mx);
+    const int e = finite_bits(__float_as_uint(mx)) ? fit_exp(mx) : 0;
+    const float f = pk::pow2i(-e);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[s][i] *= f;
+        split8(v[s], qh[s], ql[s]);
     }
-    __syncthreads();
-    // Rows that some query attends, and those that all do.
-    int hi_any = -1, lo_any = 0x7fffffff, hi_all = 0x7fffffff, lo_all = 0;
-    {
-        const int r = lane < BM ? lane : 0;
-        const int p = s_pos[r], f = s_first[r];
-        hi_any = p;
-        lo_any = f;
-        const bool real = r0 + r < r1;
-        hi_all = real ? p : 0x7fffffff;
-        lo_all = real ? f : 0;
+    const bool live = have && (unsigned)p < (unsigned)a.max_seq;
+    pos = live ? p : -1;
+    first = !live ? 0x7fffffff : a.window > 0 ? max(p + 1 - a.window, 0) : 0;
+    fq = pk::pow2i(e);
+}
+
+__device__ __forceinline__ int wave_max_i(int x) {
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            hi_any = max(hi_any, __shfl_xor(hi_any, off));
-            lo_any = min(lo_any, __shfl_xor(lo_any, off));
-            hi_all = min(hi_all, __shfl_xor(hi_all, off));
-            lo_all = max(lo_all, __shfl_xor(lo_all, off));
-        }
-        hi_any = __builtin_amdgcn_readfirstlane(hi_any) + 1;
-        lo_any = __builtin_amdgcn_readfirstlane(lo_any);
-        hi_all = __builtin_amdgcn_readfirstlane(hi_all) + 1;
-        lo_all = __builtin_amdgcn_readfirstlane(lo_all);
-    }
-    // The item's rows [lo, hi) and this split's tiles of them.
-    const int lo = OWN ? max(a.prefix, lo_any) : lo_any;
-    const int hi = OWN ? hi_any : min(a.prefix, hi_any);
-    int t_lo, t_hi;
+    for (int off = 1; off < 64; off <<= 1) x = max(x, __shfl_xor(x, off));
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
+// The tiles [lo, hi) of one split of an item's rows [row_lo, row_hi).
+template <bool OWN>
+__device__ __forceinline__ void split_tiles(const AttnArgs& a, int row_lo, int row_hi, int split, int& lo, int& hi) {
+    const int first = min(row_lo, row_hi) / kTile, end = row_lo < row_hi ? (row_hi + kTile - 1) / kTile : first;
     if constexpr (OWN) {
-        const int first = min(lo, hi) / kTile, all = lo < hi ? (hi + kTile - 1) / kTile - first : 0;
-        const int per = (all + a.own_splits - 1) / a.own_splits;
-        t_lo = first + min(split * per, all);
-        t_hi = first + min(split * per + per, all);
+        const int per = (end - first + a.own_splits - 1) / a.own_splits;
+        lo = min(first + split * per, end);
+        hi = min(lo + per, end);
     } else {
-        t_lo = max(split * a.prefix_tiles, min(lo, hi) / kTile);
-        t_hi = lo < hi ? min(split * a.prefix_tiles + a.prefix_tiles, (hi + kTile - 1) / kTile) : t_lo;
+        lo = max(split * a.prefix_tiles, first);
+        hi = max(min(split * a.prefix_tiles + a.prefix_tiles, end), lo);
     }
+}
 
-    float m[MT], l[MT], fq[MT];
-    floatx4 o[MT][DT];
+// Scores to probabilities of one tile.  st: S^T in units of 1 / (fkr * fq); on return ph, pl hold the
+// split of p = 2^(s - m).  The maxima are only raised where a score passes the present one by 2^12 or more
+// (p stays below 2^12, which fp16 holds), so that most tiles leave o as it is: true where o has to be
+// multiplied by alpha.  poison: rows of the tile that make a NaN of what attends them.
+template <int MT, class Attended>
+__device__ __forceinline__ bool tile_softmax(const AttnArgs& a, floatx4 (&st)[MT][2], float fkr, const float (&fq)[MT],
+                                             float (&m)[MT], float (&l)[MT], float (&alpha)[MT], f16x8 (&ph)[MT],
+                                             f16x8 (&pl)[MT], bool masked, unsigned poison, int g, const Attended& attended) {
+    float fs[MT], mx[MT];
+    bool up = false;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        m[mt] = kNegBig;
-        l[mt] = 0.0f;
-        fq[mt] = s_fq[16 * mt + n];
+        fs[mt] = fminf(fmaxf(fkr * fq[mt], 1.2e-38f), 1.7e38f);   // (0 * -inf would be a NaN)
+        if (a.softcap > 0.0f) {
+            const float isc = a.inv_softcap * fs[mt];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[mt][d] = floatx4{0, 0, 0, 0};
-    }
-    int ev = -1000;   // exponent that V is divided by: grows with the largest value seen
-    const int rmask = (1 << a.pool.shift) - 1;
-    const f16x8* qf = reinterpret_cast<const f16x8*>(s_q);
-    T t;
-    for (int tile = t_lo + wave; tile < t_hi; tile += kAttnWaves) {
-        const int k0 = tile * kTile;
-        // Each half tile of 16 rows lies in one page.  A block entry outside the pool holds no rows.
-        int page[2];
-        bool there[2];
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int j = (k0 + 16 * u) >> a.pool.shift;
-            page[u] = j < a.width ? __builtin_amdgcn_readfirstlane(blk[j]) : -1;
-            there[u] = paged_page_ok(page[u], a.pool.n_pages);
-            if (!there[u]) page[u] = 0;
+                for (int i = 0; i < 4; ++i) st[mt][u][i] = a.softcap_log2e * tanhf(st[mt][u][i] * isc);
+            fs[mt] = 1.0f;
         }
-        const int r0k = k0 & rmask, r1k = (k0 + 16) & rmask;
-        t.load_k(a.pool, page[0], page[1], h, r0k, r1k, n, g);
-        t.load_v(a.pool, page[0], page[1], h, r0k, r1k, n, g);
-        const bool inner = k0 >= lo && k0 + kTile <= hi && there[0] && there[1];
-        const bool plain = inner && k0 >= lo_all && k0 + kTile <= hi_all;
+        if (masked) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = 16 * u + 4 * g + i;
+                    const float x = poison >> row & 1 ? __builtin_nanf("") : st[mt][u][i];
+                    st[mt][u][i] = attended(mt, row) ? x : -__builtin_inff();
+                }
+        }
+        float x = kNegBig;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x = fmaxf(x, st[mt][u][i]);
+        x = dk::lane_step<16, true>(x);
+        x = dk::lane_step<32, true>(x);
+        mx[mt] = x * fs[mt];
+        up |= mx[mt] > m[mt] + 12.0f;
+    }
+    const bool rescale = __ballot(up) != 0;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const float mn = rescale ? fmaxf(m[mt], mx[mt] - kPShift) : m[mt];
+        alpha[mt] = dk::fast_exp2(m[mt] - mn);
+        m[mt] = mn;
+        float p[8], sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[4 * u + i] = dk::fast_exp2(__builtin_fmaf(st[mt][u][i], fs[mt], -mn));
+                sum += p[4 * u + i];
+            }
+        l[mt] = __builtin_fmaf(l[mt], alpha[mt], sum);
+        split8(p, ph[mt], pl[mt]);
+    }
+    return rescale;
+}
+
+// The factor that follows V's exponent: ev grows with the largest value seen.
+__device__ __forceinline__ float raise_exp(int& ev, int evt) {
+    const float f = evt <= ev ? 1.0f : ev < -500 ? 0.0f : pk::pow2i(max(ev - evt, -126));
+    ev = max(ev, evt);
+    return f;
+}
+
+// One tile of 16 query rows' state (o: lane's dims as D[4g + i][n] of each output tile) to its part.
+template <int D>
+__device__ __forceinline__ void store_part(const AttnArgs& a, const ItemRows& x, int r, int h, long long part, float m, float l,
+                                           const floatx4 (&o)[D / 16], int g) {
+    constexpr int NC = D / 64, REM = D % 64 / 32;
+    if (r >= x.r1) return;
+    const long long rows = (long long)a.n_tokens * a.n_heads;
+    const long long row = (long long)(x.tok0 + r / a.group) * a.n_heads + h * a.group + r % a.group;
+    if (g == 0) *reinterpret_cast<float2*>(a.part_ml + (part * rows + row) * 2) = make_float2(m, l);
+    if (l == 0.0f) return;   // (the combine takes no outputs of such a part)
+    float* po = a.part_o + (part * rows + row) * D;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<floatx4*>(po + 64 * c + 16 * g + 4 * i) =
+                floatx4{o[4 * c][i], o[4 * c + 1][i], o[4 * c + 2][i], o[4 * c + 3][i]};
+    if constexpr (REM) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float2*>(po + 64 * NC + 2 * (4 * g + i)) = make_float2(o[4 * NC][i], o[4 * NC + 1][i]);
+    }
+}
+
+// 16 query rows against a split of the prefix, or (OWN) of one sequence's own rows; the waves take the
+// split's tiles in turn.
+template <int D, bool Q8, bool OWN>
+__device__ __forceinline__ void attn_narrow(const AttnArgs& a, uint4* lds, int item, int h, int split) {
+    using T = Tile<D, Q8>;
+    constexpr int KS = D / 32, DT = D / 16;
+    // K and V of a tile in registers at once, where they leave room for two waves per SIMD.
+    constexpr bool BOTH = D <= 128 || Q8;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const ItemRows x = item_rows<OWN>(a, item, 16, lane);
+    if (x.r0 >= x.r1) return;
+    f16x8 qh[KS], ql[KS];
+    float fq[1], m[1] = {kNegBig}, l[1] = {0.0f}, alpha[1];
+    int pos, first;
+    load_queries<D>(a, x, x.r0 + n, h, g, qh, ql, fq[0], pos, first);
+    // Rows that some query attends, and those that all do.
+    const bool real = x.r0 + n < x.r1;
+    const int hi_any = wave_max_i(pos) + 1, lo_any = -wave_max_i(-first);
+    const int hi_all = -wave_max_i(real ? -pos : -0x7ffffffe) + 1, lo_all = wave_max_i(real ? first : 0);
+    const int lo = OWN ? max(a.prefix, lo_any) : lo_any, hi = OWN ? hi_any : min(a.prefix, hi_any);
+    int t_lo, t_hi;
+    split_tiles<OWN>(a, lo, hi, split, t_lo, t_hi);
+
+    floatx4 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = floatx4{0, 0, 0, 0};
+    int ev = -1000;
+    const int rmask = (1 << a.pool.shift) - 1;
+    // Entries of the block table for the two half tiles of 16 rows, each of which lies in one page; one
+    // outside the pool holds no rows (page 0 is read instead and masked).
+    auto entry = [&](int tile, int u) { return x.blk[min((tile * kTile + 16 * u) >> a.pool.shift, a.width - 1)]; };
+    auto in_pool = [&](int e) { return paged_page_ok(e, a.pool.n_pages); };
+    // Software pipeline: a tile's K is loaded behind the scores of the tile before and lands during
+    // its softmax and second product; its V is loaded behind that product and lands during the scores.
+    // The table entries are one tile further ahead.
+    T t;
+    int tile = t_lo + wave;
+    int n0 = 0, n1 = 0, c0 = 0, c1 = 0;
+    auto load_k = [&](int at) {
+        t.load_k(a.pool, in_pool(c0) ? c0 : 0, in_pool(c1) ? c1 : 0, h, at * kTile & rmask, (at * kTile + 16) & rmask, n, g);
+    };
+    auto load_v = [&](int at, int d0, int d1) {
+        t.load_v(a.pool, in_pool(d0) ? d0 : 0, in_pool(d1) ? d1 : 0, h, at * kTile & rmask, (at * kTile + 16) & rmask, n, g);
+    };
+    if (tile < t_hi) {
+        const int e0 = entry(tile, 0), e1 = entry(tile, 1);
+        n0 = entry(tile + kAttnWaves, 0);
+        n1 = entry(tile + kAttnWaves, 1);
+        c0 = __builtin_amdgcn_readfirstlane(e0);
+        c1 = __builtin_amdgcn_readfirstlane(e1);
+        load_k(tile);
+        if constexpr (BOTH) load_v(tile, c0, c1);
+    }
+    for (; tile < t_hi; tile += kAttnWaves) {
+        const int k0 = tile * kTile, v0 = c0, v1 = c1;
+        const bool there0 = in_pool(c0), there1 = in_pool(c1);
+        const bool plain = k0 >= max(lo, lo_all) && k0 + kTile <= min(hi, hi_all) && there0 && there1;
+        auto held = [&](int row) {   // row of the tile: whether the item has it
+            return (row < 16 ? there0 : there1) && k0 + row >= lo && k0 + row < hi;
+        };
+        auto attended = [&](int, int row) { return held(row) && k0 + row >= first && k0 + row <= pos; };
         unsigned poison = 0;   // rows (bit = row of the tile) that hold a value that is not finite
         if (!plain) {
-            unsigned ok = 0;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int key = k0 + 16 * u + n;
-                ok |= (unsigned)(there[u] && key >= lo && key < hi) << u;
-            }
-            const unsigned bk = t.clean_k(ok);
-            ok = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                ok |= (unsigned)(there[j >> 2] && key >= lo && key < hi) << j;
-            }
-            const unsigned bv = t.clean_v(ok);
-            if (__ballot(bk | bv) != 0) poison = tile_rows(bk, bv, n, g);
+            const unsigned bk = t.clean_k((unsigned)held(n) | (unsigned)held(16 + n) << 1);
+            if (__ballot(bk) != 0) poison = tile_rows(bk, 0, n, g);
         }
         float mk = wave_max(t.max_k());
         if (!finite_bits(__float_as_uint(mk))) {   // an infinity must not take the other rows' bits
@@ -472,85 +563,418 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(AttnArgs a) {
         }
         const int ek = fit_exp(mk);
         const float fk = pk::pow2i(-ek), fkr = pk::pow2i(ek);
-        // S^T of both half tiles, in units of 2^(ek + eq).
-        floatx4 st[MT][2];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) st[mt][0] = st[mt][1] = floatx4{0, 0, 0, 0};
+        floatx4 st[1][2] = {{{0, 0, 0, 0}, {0, 0, 0, 0}}};
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                float x[8];
-                t.k_values(u, s, fk, x);
+                float y[8];
+                t.k_values(u, s, fk, y);
                 f16x8 kh, kl;
-                split8(x, kh, kl);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const f16x8 qh = qf[((mt * KS + s) * 2 + 0) * 64 + lane], ql = qf[((mt * KS + s) * 2 + 1) * 64 + lane];
-                    st[mt][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh, st[mt][u], 0, 0, 0);
-                    st[mt][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql, st[mt][u], 0, 0, 0);
-                    st[mt][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh, st[mt][u], 0, 0, 0);
-                }
+                split8(y, kh, kl);
+                st[0][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[s], st[0][u], 0, 0, 0);
+                st[0][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[s], st[0][u], 0, 0, 0);
+                st[0][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[s], st[0][u], 0, 0, 0);
             }
-        // V's exponent: the largest of the wave's tiles so far; what is summed follows it.
+        const int next = tile + kAttnWaves;
+        if constexpr (!BOTH) load_v(tile, v0, v1);
+        c0 = __builtin_amdgcn_readfirstlane(n0);
+        c1 = __builtin_amdgcn_readfirstlane(n1);
+        if (next < t_hi) {
+            n0 = entry(next + kAttnWaves, 0);
+            n1 = entry(next + kAttnWaves, 1);
+            if constexpr (BOTH) load_k(next);
+        }
+        f16x8 ph[1], pl[1];
+        bool rescale = tile_softmax<1>(a, st, fkr, fq, m, l, alpha, ph, pl, !plain || poison, poison, g, attended);
+        unsigned bv = 0;
+        if (!plain) {
+            unsigned ok = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ok |= (unsigned)held(16 * (j >> 2) + 4 * g + (j & 3)) << j;
+            bv = t.clean_v(ok);
+        }
         float mv = wave_max(t.max_v());
         if (!finite_bits(__float_as_uint(mv))) {
-            poison |= tile_rows(0, t.clean_v(255u), n, g);
+            bv |= t.clean_v(255u);
             mv = wave_max(t.max_v());
         }
-        const int evt = fit_exp(mv);
-        float fo = 1.0f;
-        if (evt > ev) {
-            fo = ev < -500 ? 0.0f : pk::pow2i(max(ev - evt, -126));
-            ev = evt;
+        if (__ballot(bv) != 0) {
+            // a lane's rows of P are its rows of V: their probabilities become NaN where attended
+            poison = tile_rows(0, bv, n, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = 16 * (j >> 2) + 4 * g + (j & 3);
+                if ((poison >> row & 1) && attended(0, row)) {
+                    ph[0][j] = (_Float16)__builtin_nanf("");
+                    l[0] = __builtin_nanf("");
+                }
+            }
+        }
+        const float fe = raise_exp(ev, fit_exp(mv));
+        if (rescale || fe != 1.0f) {
+            const float f = alpha[0] * fe;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] = o[d] * f;
         }
         const float fv = pk::pow2i(-ev);
-        f16x8 ph[MT], pl[MT];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const float f = fkr * fq[mt];
-            float mx = kNegBig;
+        for (int tt = 0; tt < DT; ++tt) {
+            float y[8];
+            t.v_values(tt, fv, y);
+            f16x8 vh, vl;
+            split8(y, vh, vl);
+            o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[0], o[tt], 0, 0, 0);
+            o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[0], o[tt], 0, 0, 0);
+            o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[0], o[tt], 0, 0, 0);
+        }
+        if (next < t_hi) {
+            if constexpr (BOTH) load_v(next, c0, c1);
+            else load_k(next);
+        }
+    }
+    // l is a sum over the lane's own rows so far: the four groups of a query together.
+    l[0] = dk::lane_step<16, false>(l[0]);
+    l[0] = dk::lane_step<32, false>(l[0]);
+    const float f = ev < -500 ? 0.0f : pk::pow2i(ev);
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+    for (int d = 0; d < DT; ++d) o[d] = o[d] * f;
+    // The waves' states, in a fixed order: 2 into 0 and 3 into 1, then 1 into 0.
+    constexpr int XS = D / 4 + 2;
+    float* xch = reinterpret_cast<float*>(lds);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = st[mt][u][i] * f;
-                    if (a.softcap > 0.0f) x = a.softcap_log2e * tanhf(x * a.inv_softcap);
-                    if (!plain || poison) {
-                        const int key = k0 + 16 * u + 4 * g + i;
-                        const bool ok = there[u] && key >= lo && key < hi && key >= s_first[16 * mt + n] && key <= s_pos[16 * mt + n];
-                        if (poison >> (16 * u + 4 * g + i) & 1) x = __builtin_nanf("");
-                        x = ok ? x : -__builtin_inff();
+    for (int round = 0; round < 2; ++round) {
+        const int from = round == 0 ? 2 : 1, count = round == 0 ? 2 : 1;
+        if (wave >= from && wave < from + count) {
+            float* y = xch + (size_t)(wave - from) * XS * 64 + lane;
+            y[0] = m[0];
+            y[64] = l[0];
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[(2 + 4 * d + i) * 64] = o[d][i];
+        }
+        __syncthreads();
+        if (wave < count) {
+            const float* y = xch + (size_t)wave * XS * 64 + lane;
+            const float m2 = y[0], l2 = y[64];
+            const float mn = fmaxf(m[0], m2), f1 = dk::fast_exp2(m[0] - mn), f2 = dk::fast_exp2(m2 - mn);
+            m[0] = mn;
+            l[0] = l[0] * f1 + l2 * f2;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][i] = o[d][i] * f1 + y[(2 + 4 * d + i) * 64] * f2;
+        }
+        __syncthreads();
+    }
+    if (wave == 0)
+        store_part<D>(a, x, x.r0 + n, h, OWN ? a.prefix_splits + split : split, m[0], l[0], o, g);
+}
+
+// ---- a tile shared by four waves ---------------------------------------------------------------
+// In LDS: K as [2 half tiles x D/32 steps][hi, lo][lane] and V as [D/16 output tiles][hi, lo][lane], 16
+// bytes a lane, exactly the operands: every read is one conflict-free b128.  A wave loads, cleans and
+// splits the K operands p = wave, wave + 4, ... and the V units (64 dims, half tile) likewise; a unit's
+// lane holds 4 rows of 4 dims, 8 bytes of four operands.
+template <int D, bool Q8>
+struct TilePart {
+    static constexpr int KS = D / 32, NC = D / 64, REM = D % 64 / 32;
+    static constexpr int NK = 2 * KS, NV = 2 * (NC + REM);
+    static constexpr int KP = (NK + 3) / 4, VP = (NV + 3) / 4;
+    static constexpr int kBytes = (NK + D / 16) * 2 * 64 * 16;
+    floatx4 k[KP][2];      // Q8: 8 quants in the first two words, the scale in the third
+    floatx4 v[VP][4];      // Q8: 4 quants and their scale
+
+    __device__ __forceinline__ void load(const PoolPlanes& p, int page0, int page1, int h, int r0, int r1, int wave, int n, int g) {
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+            const int q = wave + 4 * i;
+            if (NK % 4 != 0 && q >= NK) break;
+            const int u = q / KS, s = q % KS, page = u ? page1 : page0, row = (u ? r1 : r0) + n;
+            if constexpr (Q8) {
+                const uint2 w = *reinterpret_cast<const uint2*>(page_row<signed char>(p.k, p, page, h, row, D) + 32 * s + 8 * g);
+                k[i][0] = floatx4{__uint_as_float(w.x), __uint_as_float(w.y), page_row<float>(p.ks, p, page, h, row, KS)[s], 0};
+            } else {
+                const float* x = page_row<float>(p.k, p, page, h, row, D) + 32 * s + 8 * g;
+                k[i][0] = *reinterpret_cast<const floatx4*>(x);
+                k[i][1] = *reinterpret_cast<const floatx4*>(x + 4);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VP; ++i) {
+            const int q = wave + 4 * i;
+            if (NV % 4 != 0 && q >= NV) break;
+            const int c = q >> 1, page = q & 1 ? page1 : page0, row = (q & 1 ? r1 : r0) + 4 * g;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (Q8) {
+                    const signed char* x = page_row<signed char>(p.v, p, page, h, row + j, D) + 64 * c;
+                    const unsigned w = c < NC ? *reinterpret_cast<const unsigned*>(x + 4 * n)
+                                              : *reinterpret_cast<const unsigned short*>(x + 2 * n);
+                    const int b = c < NC ? 2 * c + (n >> 3) : 2 * NC;
+                    v[i][j] = floatx4{__uint_as_float(w), page_row<float>(p.vs, p, page, h, row + j, KS)[b], 0, 0};
+                } else {
+                    const float* x = page_row<float>(p.v, p, page, h, row + j, D) + 64 * c;
+                    if (REM == 0 || c < NC) {
+                        v[i][j] = *reinterpret_cast<const floatx4*>(x + 4 * n);
+                    } else {
+                        const float2 w = *reinterpret_cast<const float2*>(x + 2 * n);
+                        v[i][j] = floatx4{w.x, w.y, 0, 0};
                     }
-                    st[mt][u][i] = x;
-                    mx = fmaxf(mx, x);
                 }
-            mx = dk::lane_step<16, true>(mx);
-            mx = dk::lane_step<32, true>(mx);
-            const float mn = fmaxf(m[mt], mx - kPShift);
-            const float alpha = dk::fast_exp2(m[mt] - mn);
-            m[mt] = mn;
-            float sum = 0.0f;
-            float p[8];
+            }
+        }
+    }
+    // Takes out what no row holds (held(row) false) and what is not finite; returns the rows (bit = row
+    // of the tile) of the lane's share that held such a value.
+    template <class Held>
+    __device__ __forceinline__ unsigned clean(const Held& held, int wave, int n, int g) {
+        using C = Tile<D, false>;
+        unsigned bad = 0;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+        for (int i = 0; i < KP; ++i) {
+            const int q = wave + 4 * i;
+            if (NK % 4 != 0 && q >= NK) break;
+            const int row = 16 * (q / KS) + n;
+            const unsigned keep = 0u - (unsigned)held(row);
+            unsigned worst = 0;
+            if constexpr (Q8) {
+                k[i][0][2] = C::clean(k[i][0][2], keep, worst);
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[4 * u + i] = dk::fast_exp2(st[mt][u][i] - mn);
-                    sum += p[4 * u + i];
+                for (int e = 0; e < 8; ++e) k[i][e >> 2][e & 3] = C::clean(k[i][e >> 2][e & 3], keep, worst);
+            }
+            bad |= (unsigned)(worst >= 0x7F800000u) << row;
+        }
+#pragma unroll
+        for (int i = 0; i < VP; ++i) {
+            const int q = wave + 4 * i;
+            if (NV % 4 != 0 && q >= NV) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int row = 16 * (q & 1) + 4 * g + j;
+                const unsigned keep = 0u - (unsigned)held(row);
+                unsigned worst = 0;
+                if constexpr (Q8) {
+                    v[i][j][1] = C::clean(v[i][j][1], keep, worst);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[i][j][e] = C::clean(v[i][j][e], keep, worst);
                 }
-            l[mt] = __builtin_fmaf(l[mt], alpha, sum);
-            split8(p, ph[mt], pl[mt]);
-            const float ao = alpha * fo;
+                bad |= (unsigned)(worst >= 0x7F800000u) << row;
+            }
+        }
+        return bad;
+    }
+    __device__ __forceinline__ float max_k(int wave) const {
+        float x = 0.0f;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[mt][d] = o[mt][d] * ao;
+        for (int i = 0; i < KP; ++i) {
+            if (NK % 4 != 0 && wave + 4 * i >= NK) break;
+            if constexpr (Q8) {
+                x = fmaxf(x, fabsf(k[i][0][2]) * 128.0f);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x = fmaxf(x, fabsf(k[i][e >> 2][e & 3]));
+            }
+        }
+        return x;
+    }
+    __device__ __forceinline__ float max_v(int wave) const {
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VP; ++i) {
+            if (NV % 4 != 0 && wave + 4 * i >= NV) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (Q8) {
+                    x = fmaxf(x, fabsf(v[i][j][1]) * 128.0f);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x = fmaxf(x, fabsf(v[i][j][e]));
+                }
+            }
+        }
+        return x;
+    }
+    static __device__ __forceinline__ float quant(float word, int byte) {
+        return (float)(signed char)(__float_as_uint(word) >> (8 * byte) & 0xFF);
+    }
+    __device__ __forceinline__ void store(uint4* lds, float fk, float fv, int wave, int lane) const {
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+            const int q = wave + 4 * i;
+            if (NK % 4 != 0 && q >= NK) break;
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] = Q8 ? quant(k[i][0][e >> 2], e & 3) * (k[i][0][2] * fk) : k[i][e >> 2][e & 3] * fk;
+            f16x8 hi, lo;
+            split8(x, hi, lo);
+            lds[(2 * q + 0) * 64 + lane] = __builtin_bit_cast(uint4, hi);
+            lds[(2 * q + 1) * 64 + lane] = __builtin_bit_cast(uint4, lo);
+        }
+        uint2* lv = reinterpret_cast<uint2*>(lds + NK * 2 * 64);
+#pragma unroll
+        for (int i = 0; i < VP; ++i) {
+            const int q = wave + 4 * i;
+            if (NV % 4 != 0 && q >= NV) break;
+            const int c = q >> 1;
+#pragma unroll
+            for (int t = 0; t < 4; t += 2) {   // columns t and t + 1
+                if (REM && c >= NC && t > 0) break;
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int w = 0; w < 2; ++w)
+                        x[4 * w + j] = Q8 ? quant(v[i][j][0], t + w) * (v[i][j][1] * fv) : v[i][j][t + w] * fv;
+                f16x8 hi, lo;
+                split8(x, hi, lo);
+                const uint4 uh = __builtin_bit_cast(uint4, hi), ul = __builtin_bit_cast(uint4, lo);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const int tt = 4 * c + t + w;
+                    lv[((2 * tt + 0) * 64 + lane) * 2 + (q & 1)] = w ? make_uint2(uh.z, uh.w) : make_uint2(uh.x, uh.y);
+                    lv[((2 * tt + 1) * 64 + lane) * 2 + (q & 1)] = w ? make_uint2(ul.z, ul.w) : make_uint2(ul.x, ul.y);
+                }
+            }
+        }
+    }
+};
+
+// 64*MT query rows, 16*MT a wave, against a split of the prefix, or (OWN) of one sequence's own rows.
+template <int D, int MT, bool Q8, bool OWN>
+__device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int item, int h, int split) {
+    using T = TilePart<D, Q8>;
+    constexpr int KS = D / 32, DT = D / 16, NK = T::NK;
+    __shared__ int s_range[2][kAttnWaves];
+    __shared__ float s_max[2][kAttnWaves];
+    __shared__ unsigned s_bad[kAttnWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
+    const ItemRows x = item_rows<OWN>(a, item, 64 * MT, lane);
+    if (x.r0 >= x.r1) return;
+    const int rw = x.r0 + 16 * MT * wave;
+    f16x8 qh[MT][KS], ql[MT][KS];
+    float fq[MT], m[MT], l[MT], alpha[MT];
+    int pos[MT], first[MT], hi_any = -1, lo_any = 0x7fffffff, hi_all = 0x7ffffffe, lo_all = 0;
+    floatx4 o[MT][DT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int r = rw + 16 * mt + n;
+        load_queries<D>(a, x, r, h, g, qh[mt], ql[mt], fq[mt], pos[mt], first[mt]);
+        hi_any = max(hi_any, pos[mt]);
+        lo_any = min(lo_any, first[mt]);
+        if (r < x.r1) {
+            hi_all = min(hi_all, pos[mt]);
+            lo_all = max(lo_all, first[mt]);
+        }
+        m[mt] = kNegBig;
+        l[mt] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[mt][d] = floatx4{0, 0, 0, 0};
+    }
+    hi_any = wave_max_i(hi_any) + 1;
+    lo_any = -wave_max_i(-lo_any);
+    hi_all = -wave_max_i(-hi_all) + 1;
+    lo_all = wave_max_i(lo_all);
+    if (lane == 0) {
+        s_range[0][wave] = lo_any;
+        s_range[1][wave] = hi_any;
+    }
+    __syncthreads();
+    int lo = s_range[0][0], hi = s_range[1][0];
+#pragma unroll
+    for (int w = 1; w < kAttnWaves; ++w) {
+        lo = min(lo, s_range[0][w]);
+        hi = max(hi, s_range[1][w]);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    if constexpr (OWN) lo = max(a.prefix, lo);
+    else hi = min(a.prefix, hi);
+    int t_lo, t_hi;
+    split_tiles<OWN>(a, lo, hi, split, t_lo, t_hi);
+
+    int ev = -1000;
+    const int rmask = (1 << a.pool.shift) - 1;
+    auto entry = [&](int tile, int u) { return x.blk[min((tile * kTile + 16 * u) >> a.pool.shift, a.width - 1)]; };
+    auto in_pool = [&](int e) { return paged_page_ok(e, a.pool.n_pages); };
+    T t;
+    int n0 = 0, n1 = 0, c0 = 0, c1 = 0;
+    auto load = [&](int at) {
+        t.load(a.pool, in_pool(c0) ? c0 : 0, in_pool(c1) ? c1 : 0, h, at * kTile & rmask, (at * kTile + 16) & rmask, wave, n, g);
+    };
+    if (t_lo < t_hi) {
+        const int e0 = entry(t_lo, 0), e1 = entry(t_lo, 1);
+        n0 = entry(t_lo + 1, 0);
+        n1 = entry(t_lo + 1, 1);
+        c0 = __builtin_amdgcn_readfirstlane(e0);
+        c1 = __builtin_amdgcn_readfirstlane(e1);
+        load(t_lo);
+    }
+    const f16x8* op = reinterpret_cast<const f16x8*>(lds);
+    for (int tile = t_lo; tile < t_hi; ++tile) {
+        const int k0 = tile * kTile;
+        const bool there0 = in_pool(c0), there1 = in_pool(c1);
+        auto held = [&](int row) { return (row < 16 ? there0 : there1) && k0 + row >= lo && k0 + row < hi; };
+        const bool whole = k0 >= lo && k0 + kTile <= hi && there0 && there1;
+        // Whether every wave's queries attend all of the tile is the wave's own matter (plain, below);
+        // a value that is not finite has to be taken out wherever some query does not attend its row.
+        unsigned bad = t.clean(held, wave, n, g);
+        const float mk = wave_max(t.max_k(wave)), mv = wave_max(t.max_v(wave));
+        bad = __ballot(bad) != 0 ? wave_or(bad) : 0u;
+        if (lane == 0) {
+            s_max[0][wave] = mk;
+            s_max[1][wave] = mv;
+            s_bad[wave] = bad;
+        }
+        __syncthreads();   // and the last reads of the tile before
+        const float ak = fmaxf(fmaxf(s_max[0][0], s_max[0][1]), fmaxf(s_max[0][2], s_max[0][3]));
+        const float av = fmaxf(fmaxf(s_max[1][0], s_max[1][1]), fmaxf(s_max[1][2], s_max[1][3]));
+        const unsigned poison = __builtin_amdgcn_readfirstlane(s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]);
+        const int ek = __builtin_amdgcn_readfirstlane(fit_exp(ak));
+        const float fe = raise_exp(ev, __builtin_amdgcn_readfirstlane(fit_exp(av)));
+        t.store(lds, pk::pow2i(-ek), pk::pow2i(-ev), wave, lane);
+        c0 = __builtin_amdgcn_readfirstlane(n0);
+        c1 = __builtin_amdgcn_readfirstlane(n1);
+        if (tile + 1 < t_hi) {
+            n0 = entry(tile + 2, 0);
+            n1 = entry(tile + 2, 1);
+            load(tile + 1);
+        }
+        __syncthreads();
+        if (rw >= x.r1) continue;   // no rows of its own: only the loads are its work
+        floatx4 st[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) st[mt][0] = st[mt][1] = floatx4{0, 0, 0, 0};
+#pragma unroll
+        for (int q = 0; q < NK; ++q) {
+            const f16x8 kh = op[2 * q * 64 + lane], kl = op[(2 * q + 1) * 64 + lane];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                floatx4& c = st[mt][q / KS];
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[mt][q % KS], c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[mt][q % KS], c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[mt][q % KS], c, 0, 0, 0);
+            }
+        }
+        const bool plain = whole && k0 >= lo_all && k0 + kTile <= hi_all;
+        auto attended = [&](int mt, int row) { return held(row) && k0 + row >= first[mt] && k0 + row <= pos[mt]; };
+        f16x8 ph[MT], pl[MT];
+        const bool rescale = tile_softmax<MT>(a, st, pk::pow2i(ek), fq, m, l, alpha, ph, pl, !plain || poison, poison, g, attended);
+        if (rescale || fe != 1.0f) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float f = alpha[mt] * fe;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[mt][d] = o[mt][d] * f;
+            }
         }
 #pragma unroll
         for (int tt = 0; tt < DT; ++tt) {
-            float x[8];
-            t.v_values(tt, fv, x);
-            f16x8 vh, vl;
-            split8(x, vh, vl);
+            const f16x8 vh = op[(NK + tt) * 2 * 64 + lane], vl = op[((NK + tt) * 2 + 1) * 64 + lane];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[mt], o[mt][tt], 0, 0, 0);
@@ -559,102 +983,129 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(AttnArgs a) {
             }
         }
     }
-    // l is a sum over the lane's own rows so far: the four groups of a query together.
+    const float f = ev < -500 ? 0.0f : pk::pow2i(ev);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         l[mt] = dk::lane_step<16, false>(l[mt]);
         l[mt] = dk::lane_step<32, false>(l[mt]);
-        const float f = ev < -500 ? 0.0f : pk::pow2i(ev);
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[mt][d] = o[mt][d] * f;
-    }
-    // The waves' states, in a fixed order: 2 into 0 and 3 into 1, then 1 into 0.
-    __syncthreads();   // the last reads of the queries
-    constexpr int XS = MT * (D / 4 + 2);
-    float* xch = reinterpret_cast<float*>(s_dyn4);
-#pragma unroll
-    for (int round = 0; round < 2; ++round) {
-        const int from = round == 0 ? 2 : 1, count = round == 0 ? 2 : 1;
-        if (wave >= from && wave < from + count) {
-            float* x = xch + (size_t)(wave - from) * XS * 64 + lane;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                x[(mt * (D / 4 + 2) + 0) * 64] = m[mt];
-                x[(mt * (D / 4 + 2) + 1) * 64] = l[mt];
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[(mt * (D / 4 + 2) + 2 + 4 * d + i) * 64] = o[mt][d][i];
-            }
-        }
-        __syncthreads();
-        if (wave < count) {
-            const float* x = xch + (size_t)wave * XS * 64 + lane;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const float m2 = x[(mt * (D / 4 + 2) + 0) * 64], l2 = x[(mt * (D / 4 + 2) + 1) * 64];
-                const float mn = fmaxf(m[mt], m2), f1 = dk::fast_exp2(m[mt] - mn), f2 = dk::fast_exp2(m2 - mn);
-                m[mt] = mn;
-                l[mt] = l[mt] * f1 + l2 * f2;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        o[mt][d][i] = o[mt][d][i] * f1 + x[(mt * (D / 4 + 2) + 2 + 4 * d + i) * 64] * f2;
-            }
-        }
-        __syncthreads();
-    }
-    if (wave != 0) return;
-    const long long rows = (long long)a.n_tokens * a.n_heads;
-    const long long part = OWN ? a.prefix_splits + split : split;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const int r = r0 + 16 * mt + n;
-        if (r >= r1) continue;
-        const long long row = (long long)(tok0 + r / G) * a.n_heads + h * G + r % G;
-        if (g == 0) *reinterpret_cast<float2*>(a.part_ml + (part * rows + row) * 2) = make_float2(m[mt], l[mt]);
-        float* po = a.part_o + (part * rows + row) * D;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<floatx4*>(po + 64 * c + 16 * g + 4 * i) =
-                    floatx4{o[mt][4 * c][i], o[mt][4 * c + 1][i], o[mt][4 * c + 2][i], o[mt][4 * c + 3][i]};
-        if constexpr (REM) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<float2*>(po + 64 * NC + 2 * (4 * g + i)) = make_float2(o[mt][4 * NC][i], o[mt][4 * NC + 1][i]);
-        }
+        store_part<D>(a, x, rw + 16 * mt + n, h, OWN ? a.prefix_splits + split : split, m[mt], l[mt], o[mt], g);
     }
 }
 
-// Joins the partials of each query row (prefix splits, then own splits, in that order) and applies
-// sink and gate.  A thread takes four dims of one row.  A row with nothing to attend is zero; rows
-// of tokens behind the last sequence are left as they are.
+// Index of workgroup `id` of `count` (a multiple of 8) in an order that gives each of the chip's 8
+// parts, which take the workgroups in turn, a consecutive range: items that read the same rows follow
+// one another and share that part's L2.
+__device__ __forceinline__ int by_part(int id, int count) { return (id & 7) * (count >> 3) + (id >> 3); }
+
+// WIDE 0: items of 16 query rows; else of 64*WIDE.
+template <int D, int WIDE, bool Q8, bool OWN>
+__device__ __forceinline__ void attn_item(const AttnArgs& a, uint4* lds, int item, int h, int split) {
+    if constexpr (WIDE == 0) attn_narrow<D, Q8, OWN>(a, lds, item, h, split);
+    else attn_wide<D, WIDE, Q8, OWN>(a, lds, item, h, split);
+}
+
+// Workgroups [0, prefix_wgs) take the prefix items (block of query rows fastest, then split, then KV
+// head), the others the own rows' (item of item_sequence, split, KV head): one launch, so the one fills
+// what the other leaves of the chip.
+template <int D, int WP, int WO, bool Q8>
+__global__ __launch_bounds__(kAttnThreads, 2) void paged_attn_kernel(AttnArgs a) {
+    extern __shared__ uint4 s_dyn4[];
+    int id = blockIdx.x;
+    if (id < a.prefix_wgs) {
+        id = by_part(id, a.prefix_wgs);
+        const int item = id % a.prefix_items, hs = id / a.prefix_items;
+        if (hs >= a.pool.n_kv_heads * a.prefix_splits) return;
+        attn_item<D, WP, Q8, false>(a, s_dyn4, item, hs / a.prefix_splits, hs % a.prefix_splits);
+    } else {
+        id = by_part(id - a.prefix_wgs, (int)gridDim.x - a.prefix_wgs);
+        const int item = id % a.own_items, hs = id / a.own_items;
+        if (hs >= a.pool.n_kv_heads * a.own_splits) return;
+        attn_item<D, WO, Q8, true>(a, s_dyn4, item, hs / a.own_splits, hs % a.own_splits);
+    }
+}
+
+// Joins the partials of each query row (prefix splits, then own splits) and applies sink and gate.  A
+// group of D/4 threads (four dims each) takes one row's partials; a row with several of them is taken by
+// GR groups, every GR-th partial each, all loads in flight together, which meet in LDS in a fixed
+// order.  A row with nothing to attend is zero; rows of tokens behind the last sequence are left as they
+// are.
 constexpr int kJoinThreads = 256;
 template <int D>
+constexpr int join_groups() { return kJoinThreads / (D / 4); }
+// Groups per row for S partials: a power of two that leaves each at most about two.
+template <int D>
+__host__ __device__ constexpr int join_groups_per_row(int S) {
+    int gr = 1;
+    while (2 * gr <= join_groups<D>() && 2 * gr < S) gr *= 2;
+    return gr;
+}
+template <int D>
 __global__ __launch_bounds__(kJoinThreads) void paged_combine_kernel(AttnArgs a) {
-    constexpr int TPR = D / 4, RPB = kJoinThreads / TPR;
-    const int local = threadIdx.x / TPR, col = threadIdx.x % TPR;
-    const long long rows = (long long)a.n_tokens * a.n_heads;
-    const long long row = (long long)blockIdx.x * RPB + local;
-    if (local >= RPB || row >= rows) return;
+    constexpr int TPR = D / 4, NG = join_groups<D>(), U = 4;
+    __shared__ float2 s_ml[NG];
+    __shared__ floatx4 s_o[NG][TPR];
+    const int S = a.prefix_splits + a.own_splits, SG = join_groups_per_row<D>(S), RPB = NG / SG;
+    const int grp = threadIdx.x / TPR, col = threadIdx.x % TPR, sg = grp % SG;
+    const long long rows = (long long)a.n_tokens * a.n_heads, row = (long long)blockIdx.x * RPB + grp / SG;
     const int tok = (int)(row / a.n_heads), head = (int)(row % a.n_heads);
-    if (tok < a.seq_start[0] || tok >= a.seq_start[a.n_seqs]) return;
-    const int S = a.prefix_splits + a.own_splits;
-    float M = kNegBig;
-    for (int s = 0; s < S; ++s) M = fmaxf(M, a.part_ml[(s * rows + row) * 2]);
-    float L = 0.0f;
+    const bool mine = grp < RPB * SG && row < rows && tok >= a.seq_start[0] && tok < a.seq_start[a.n_seqs];
+    float M = kNegBig, L = 0.0f;
     floatx4 O = {0, 0, 0, 0};
-    for (int s = 0; s < S; ++s) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (s * rows + row) * 2);
-        if (ml.y == 0.0f) continue;
-        const float f = dk::fast_exp2(ml.x - M);
-        L = __builtin_fmaf(ml.y, f, L);
-        const floatx4 x = *reinterpret_cast<const floatx4*>(a.part_o + (s * rows + row) * D + 4 * col);
+    if (mine)
+        for (int s0 = sg; s0 < S; s0 += SG * U) {
+            float2 ml[U];
+            floatx4 x[U];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) O[i] = __builtin_fmaf(x[i], f, O[i]);
+            for (int u = 0; u < U; ++u) {
+                const int s = s0 + u * SG;
+                ml[u] = s < S ? *reinterpret_cast<const float2*>(a.part_ml + (s * rows + row) * 2) : make_float2(kNegBig, 0.0f);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int s = min(s0 + u * SG, S - 1);
+                x[u] = *reinterpret_cast<const floatx4*>(a.part_o + (s * rows + row) * D + 4 * col);
+            }
+            float mn = M;
+#pragma unroll
+            for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+            const float f0 = dk::fast_exp2(M - mn);
+            M = mn;
+            L *= f0;
+            O = O * f0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (ml[u].y == 0.0f) continue;   // such a part wrote no outputs
+                const float f = dk::fast_exp2(ml[u].x - M);
+                L = __builtin_fmaf(ml[u].y, f, L);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) O[i] = __builtin_fmaf(x[u][i], f, O[i]);
+            }
+        }
+    if (SG > 1) {
+        if (grp < NG) {
+            if (col == 0) s_ml[grp] = make_float2(M, L);
+            s_o[grp][col] = O;
+        }
+        __syncthreads();
+        if (!mine || sg > 0) return;
+        const int used = min(S, SG);
+        float mn = M;
+        for (int k = 1; k < used; ++k) mn = fmaxf(mn, s_ml[grp + k].x);
+        const float f0 = dk::fast_exp2(M - mn);
+        M = mn;
+        L *= f0;
+        O = O * f0;
+        for (int k = 1; k < used; ++k) {
+            const float f = dk::fast_exp2(s_ml[grp + k].x - M);
+            L = __builtin_fmaf(s_ml[grp + k].y, f, L);
+            const floatx4 x = s_o[grp + k][col];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) O[i] = __builtin_fmaf(x[i], f, O[i]);
+        }
+    } else if (!mine) {
+        return;
     }
     floatx4 r = {0, 0, 0, 0};
     if (L != 0.0f) {   // (true for NaN as well)

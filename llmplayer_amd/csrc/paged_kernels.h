@@ -165,13 +165,14 @@ __device__ __forceinline__ floatx4 load4_in(const void* p, long long i, int f32)
                    __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u)};
 }
 
-// Scale of 32 values: their largest magnitude times 1/127, in one product (a contiguous cache divides;
-// the two differ by at most one unit in the last place).
+// Scale of 32 values.  Rounded quants take the largest magnitude times 1/127, one product (within one
+// unit in the last place of the division, which moves a quant only at a border between two).  Truncated
+// ones take a contiguous cache's division: there the last place decides the quant of the largest value.
 constexpr float kInv127 = 1.0f / 127.0f;
-__device__ __forceinline__ float block_scale(const float* x) {
+__device__ __forceinline__ float block_scale(const float* x, bool trunc) {
     float mx = 0.0f;
     for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fabsf(x[i]));
-    return mx * kInv127;
+    return trunc ? mx / 127.0f : mx * kInv127;
 }
 
 // One workgroup = (token, group of kAppendHeads heads): the heads [h0, h0 + kAppendHeads) of the token's
@@ -234,7 +235,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_lds_kernel(Append
     constexpr int NB = D / 32;
     for (int b = tid + nq * NB; b < nh * NB; b += kAppendThreads) {
         const int hh = h0 + b / NB;
-        const float scale = block_scale(s_x + 32 * b);
+        const float scale = block_scale(s_x + 32 * b, a.q8_trunc != 0);
         s_inv[b] = dk::q8_inv_scale(scale);
         (hh < Hq + Hkv ? a.pool.ks : a.pool.vs)[row_of(hh) * NB + b % NB] = scale;
     }

@@ -129,35 +129,38 @@ LLMP_HD inline int paged_item_base(int start, int group, int rows, int b) {
 }
 
 // ---- launch plan -------------------------------------------------------------------------------
+// Query rows of a work item: 16 (wide 0), or 64 or 128 (wide 1, 2; at head_dim 256 the outputs of 128
+// do not fit the registers).
+LLMP_HD constexpr int paged_item_rows(int wide) { return wide ? 64 * wide : 16; }
+constexpr int paged_wide_max(int head_dim) { return head_dim > 128 ? 1 : 2; }
+
 struct PagedPlan {
-    int prefix_mt, prefix_splits, prefix_tiles;   // tiles of 16 query rows a workgroup, splits, 32-row tiles a split
-    int own_mt, own_splits;
+    int prefix_wide, prefix_splits, prefix_tiles;   // item size, splits, 32-row tiles of a split
+    int own_wide, own_splits;
 };
 
 // n_seqs and max_len (the longest sequence, a bound that the caller gives) set the size of the own
 // rows' work: nothing but the speed depends on them.
 inline PagedPlan paged_plan(int n_seqs, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int prefix, int max_len,
                             int n_cu) {
-    const long long cu = n_cu > 0 ? n_cu : 256, group = n_heads / n_kv_heads;
-    const int mt_max = head_dim > 128 ? 2 : 4;
-    auto tiles_of = [&](long long rows) { return rows <= 16 ? 1 : rows <= 32 || mt_max == 2 ? 2 : 4; };
-    PagedPlan p{};
-    // At least 8 tiles of 32 rows a split: two for each of its four waves.
+    const long long cu = n_cu > 0 ? n_cu : 256, group = n_heads / n_kv_heads, rows = (long long)n_tokens * group;
+    auto wide_of = [&](long long r) { return r <= 16 ? 0 : r <= 64 ? 1 : paged_wide_max(head_dim); };
+    auto items_of = [&](long long r, int wide) { return (r + paged_item_rows(wide) - 1) / paged_item_rows(wide); };
+    // About two workgroups a CU, with at least 8 tiles of 32 rows a split.
     auto splits_of = [&](long long tiles, long long items) {
         return (int)std::max<long long>(1, std::min((2 * cu + items - 1) / items, (tiles + 7) / 8));
     };
+    PagedPlan p{};
+    const long long each = (rows + n_seqs - 1) / n_seqs;
+    p.prefix_wide = wide_of(rows);
+    p.own_wide = wide_of(each);
     if (prefix > 0) {
-        const long long rows = (long long)n_tokens * group, tiles = (prefix + 31) / 32;
-        p.prefix_mt = tiles_of(rows);
-        const long long items = (rows + 16 * p.prefix_mt - 1) / (16 * p.prefix_mt) * n_kv_heads;
-        const int s = splits_of(tiles, items);
+        const long long tiles = (prefix + 31) / 32;
+        const int s = splits_of(tiles, items_of(rows, p.prefix_wide) * n_kv_heads);
         p.prefix_tiles = (int)((tiles + s - 1) / s);
         p.prefix_splits = (int)((tiles + p.prefix_tiles - 1) / p.prefix_tiles);
     }
-    const long long each = ((long long)n_tokens * group + n_seqs - 1) / n_seqs;
-    p.own_mt = tiles_of(each);
-    const long long items = (long long)n_seqs * ((each + 16 * p.own_mt - 1) / (16 * p.own_mt)) * n_kv_heads;
-    p.own_splits = splits_of((std::max(max_len - prefix, 1) + 31) / 32, items);
+    p.own_splits = splits_of((std::max(max_len - prefix, 1) + 31) / 32, n_seqs * items_of(each, p.own_wide) * n_kv_heads);
     return p;
 }
 

@@ -161,13 +161,13 @@ static void plans() {
                             for (int longest : {1, 33, 5001, 140000}) {
                                 const PagedPlan p = paged_plan(n, tokens, hq, hkv, d, prefix, longest, 256);
                                 CHECK(p.own_splits >= 1 && p.own_splits <= 65535);
-                                CHECK(p.own_mt == 1 || p.own_mt == 2 || (p.own_mt == 4 && d <= 128));
+                                CHECK(p.own_wide >= 0 && p.own_wide <= paged_wide_max(d) && p.own_wide <= p.prefix_wide);
+                                CHECK(p.prefix_wide <= paged_wide_max(d));
                                 if (prefix == 0) {
                                     CHECK(p.prefix_splits == 0);
                                     continue;
                                 }
                                 const int tiles = (prefix + 31) / 32;
-                                CHECK(p.prefix_mt == 1 || p.prefix_mt == 2 || (p.prefix_mt == 4 && d <= 128));
                                 CHECK(p.prefix_splits >= 1 && p.prefix_splits <= 65535);
                                 CHECK((long long)p.prefix_splits * p.prefix_tiles >= tiles);
                                 CHECK((long long)(p.prefix_splits - 1) * p.prefix_tiles < tiles);

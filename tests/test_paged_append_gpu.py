@@ -133,7 +133,7 @@ def test_append(hq, hkv, D, page, T, rope_type, rope_dim, norm, norm_mode, cache
                     rk = dict(zip(("k", "v"), ref.read(0, int(positions[t]), 1)))
                     for w in "kv":
                         x = rk[w].reshape(-1, 32)
-                        rk[w + "s"] = np.abs(x).max(1) * F32(1 / 127)
+                        rk[w + "s"] = np.abs(x).max(1) / F32(127) if cache == 2 else np.abs(x).max(1) * F32(1 / 127)
                         with np.errstate(divide="ignore"):
                             y = x * np.where(rk[w + "s"] > 0, F32(1) / rk[w + "s"], F32(0))[:, None]
                         y = np.trunc(y) if cache == 2 else np.floor(y) + (y - np.floor(y) >= F32(0.5))
