@@ -9,7 +9,10 @@ namespace {
 template <int D, int WP, int WO, bool Q8>
 hipError_t launch(pg::AttnArgs a, hipStream_t st) {
     constexpr size_t lds = std::max(pg::attn_lds<D>(WP), pg::attn_lds<D>(WO));
-    static_assert(lds <= 65536, "within what a launch has without asking");
+    // LDS above 64 KB has to be asked for, once per kernel.
+    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(&pg::paged_attn_kernel<D, WP, WO, Q8>),
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (allowed != hipSuccess) return allowed;
     const long long rows = (long long)a.n_tokens * a.group, h = a.pool.n_kv_heads;
     const long long rp = paged_item_rows(WP), ro = paged_item_rows(WO);
     const long long p = (rows + rp - 1) / rp, o = rows / ro + a.n_seqs;

@@ -42,6 +42,55 @@ constexpr int kTile = 32;            // pool rows a wave takes at a time
 constexpr float kPShift = 4.0f;      // 2^(s - m + 4): small probabilities keep their fp16 bits
 constexpr float kNegBig = dk::kNegBig;
 
+// max(m, |x|, |y|) in one instruction.  (The compiler quiets every loaded value first, one more each.)
+__device__ __forceinline__ float max_abs(float m, float x, float y) {
+    asm("v_max3_f32 %0, |%1|, |%2|, %0" : "+v"(m) : "v"(x), "v"(y));
+    return m;
+}
+
+// Split of x*f: hi = fp16(x*f), lo = fp16(x*f - hi), one mixed-precision multiply-add each, the first
+// rounded from the exact product and the second from the exact difference.
+// In plain operations, not in assembly: the compiler has to see who writes an operand of a matrix
+// instruction, which must not read it within two wait states.  The opaque step keeps lo to the `hi` that
+// was rounded above.
+__device__ __forceinline__ void split2(float x, float y, float fx, float fy, pk::f16x2& hi, pk::f16x2& lo) {
+    const pk::f16x2 r = {(_Float16)(x * fx), (_Float16)(y * fy)};
+    unsigned u = __builtin_bit_cast(unsigned, r);
+    asm("" : "+v"(u));
+    hi = __builtin_bit_cast(pk::f16x2, u);
+    lo = pk::f16x2{(_Float16)__builtin_fmaf(x, fx, -(float)hi[0]), (_Float16)__builtin_fmaf(y, fy, -(float)hi[1])};
+}
+__device__ __forceinline__ void split8(const float (&x)[8], const float (&f)[8], f16x8& hi, f16x8& lo) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        pk::f16x2 h, l;
+        split2(x[2 * j], x[2 * j + 1], f[2 * j], f[2 * j + 1], h, l);
+        hi[2 * j] = h[0];
+        hi[2 * j + 1] = h[1];
+        lo[2 * j] = l[0];
+        lo[2 * j + 1] = l[1];
+    }
+}
+__device__ __forceinline__ void split8(const float (&x)[8], float f, f16x8& hi, f16x8& lo) {
+    const float ff[8] = {f, f, f, f, f, f, f, f};
+    split8(x, ff, hi, lo);
+}
+// Probabilities: no factor.
+__device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo) {
+    float minus = -1.0f;
+    asm("" : "+s"(minus));   // (x - hi stays one multiply-add)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        unsigned u = pk::pack_f16(x[2 * j], x[2 * j + 1]);
+        asm("" : "+v"(u));
+        const pk::f16x2 h = __builtin_bit_cast(pk::f16x2, u);
+        hi[2 * j] = h[0];
+        hi[2 * j + 1] = h[1];
+        lo[2 * j] = (_Float16)__builtin_fmaf((float)h[0], minus, x[2 * j]);
+        lo[2 * j + 1] = (_Float16)__builtin_fmaf((float)h[1], minus, x[2 * j + 1]);
+    }
+}
+
 // ---- one tile of 32 rows in registers --------------------------------------------------------
 template <int D, bool Q8>
 struct Tile;
@@ -94,7 +143,7 @@ struct Tile<D, false> {
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x = fmaxf(x, fabsf(k[u][s][q][e]));
+                    for (int e = 0; e < 4; e += 2) x = max_abs(x, k[u][s][q][e], k[u][s][q][e + 1]);
         return x;
     }
     __device__ __forceinline__ float max_v() const {
@@ -104,8 +153,8 @@ struct Tile<D, false> {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x = fmaxf(x, fabsf(v[j][c][e]));
-            if constexpr (REM) x = fmaxf(x, fmaxf(fabsf(vr[j][0]), fabsf(vr[j][1])));
+                for (int e = 0; e < 4; e += 2) x = max_abs(x, v[j][c][e], v[j][c][e + 1]);
+            if constexpr (REM) x = max_abs(x, vr[j][0], vr[j][1]);
         }
         return x;
     }
@@ -152,14 +201,18 @@ struct Tile<D, false> {
         }
         return r;
     }
-    __device__ __forceinline__ void k_values(int u, int s, float f, float (&x)[8]) const {
+    __device__ __forceinline__ void k_split(int u, int s, float f, f16x8& hi, f16x8& lo) const {
+        float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = k[u][s][e >> 2][e & 3] * f;
+        for (int e = 0; e < 8; ++e) x[e] = k[u][s][e >> 2][e & 3];
+        split8(x, f, hi, lo);
     }
     // Output tile tt's column of the 8 rows.
-    __device__ __forceinline__ void v_values(int tt, float f, float (&x)[8]) const {
+    __device__ __forceinline__ void v_split(int tt, float f, f16x8& hi, f16x8& lo) const {
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (tt < 4 * NC ? v[j][tt >> 2][tt & 3] : vr[j][(tt - 4 * NC) & 1]) * f;
+        for (int j = 0; j < 8; ++j) x[j] = tt < 4 * NC ? v[j][tt >> 2][tt & 3] : vr[j][(tt - 4 * NC) & 1];
+        split8(x, f, hi, lo);
     }
 };
 
@@ -238,40 +291,24 @@ struct Tile<D, true> {
         }
         return r;
     }
-    __device__ __forceinline__ void k_values(int u, int s, float f, float (&x)[8]) const {
-        const float sc = ks[u][s] * f;
+    __device__ __forceinline__ void k_split(int u, int s, float f, f16x8& hi, f16x8& lo) const {
         const unsigned w[2] = {k[u][s].x, k[u][s].y};
+        float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (float)(signed char)(w[e >> 2] >> (8 * (e & 3)) & 0xFF) * sc;
+        for (int e = 0; e < 8; ++e) x[e] = (float)(signed char)(w[e >> 2] >> (8 * (e & 3)) & 0xFF);
+        split8(x, ks[u][s] * f, hi, lo);
     }
-    __device__ __forceinline__ void v_values(int tt, float f, float (&x)[8]) const {
+    __device__ __forceinline__ void v_split(int tt, float f, f16x8& hi, f16x8& lo) const {
         const int c = tt < 4 * NC ? tt >> 2 : NC, t = tt < 4 * NC ? tt & 3 : tt - 4 * NC;
+        float x[8], y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (float)(signed char)(v[j][c] >> (8 * t) & 0xFF) * (vs[j][c] * f);
+        for (int j = 0; j < 8; ++j) {
+            x[j] = (float)(signed char)(v[j][c] >> (8 * t) & 0xFF);
+            y[j] = vs[j][c] * f;
+        }
+        split8(x, y, hi, lo);
     }
 };
-
-// hi = fp16(x), lo = fp16(x - hi): one conversion a pair and one mixed-precision multiply-add a value.
-// In plain operations, not in assembly: the compiler has to see who writes an operand of a matrix
-// instruction, which must not read it within two wait states.  Two opaque steps keep its hands off the
-// arithmetic: `hi` as it was rounded is what lo starts from (a product may be rounded to fp16 in one
-// step for the one and in two for the other), and x - hi stays a multiply-add by a -1 it cannot see.
-__device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo) {
-    float minus = -1.0f;
-    asm("" : "+s"(minus));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        unsigned u = pk::pack_f16(x[2 * j], x[2 * j + 1]);
-        asm("" : "+v"(u));
-        const pk::f16x2 h = __builtin_bit_cast(pk::f16x2, u);
-        const pk::f16x2 l = {(_Float16)__builtin_fmaf((float)h[0], minus, x[2 * j]),
-                             (_Float16)__builtin_fmaf((float)h[1], minus, x[2 * j + 1])};
-        hi[2 * j] = h[0];
-        hi[2 * j + 1] = h[1];
-        lo[2 * j] = l[0];
-        lo[2 * j + 1] = l[1];
-    }
-}
 
 // Largest value over the wave.
 __device__ __forceinline__ float wave_max(float x) {
@@ -301,10 +338,11 @@ __device__ __forceinline__ unsigned tile_rows(unsigned bk, unsigned bv, int n, i
     return wave_or((bk & 1u) << n | (bk >> 1) << (16 + n) | (bv & 15u) << (4 * g) | (bv >> 4) << (16 + 4 * g));
 }
 
-// Dynamic LDS: the waves' states that attn_narrow joins, or attn_wide's tile.
+// Tiles that attn_wide holds, and the dynamic LDS: these, or the waves' states that attn_narrow joins.
+constexpr int wide_tiles(int D) { return D <= 128 ? 2 : 1; }
 template <int D>
 constexpr size_t attn_lds(int wide) {
-    return wide ? (size_t)(D / 16 + D / 16) * 2 * 64 * 16 : 2 * (size_t)(D / 4 + 2) * 64 * 4;
+    return wide ? (size_t)wide_tiles(D) * (D / 16 + D / 16) * 2 * 64 * 16 : 2 * (size_t)(D / 4 + 2) * 64 * 4;
 }
 
 // The sequence of work item `item` of an own-rows launch (paged_item_base).
@@ -497,7 +535,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs& a, uint4* lds, int i
     using T = Tile<D, Q8>;
     constexpr int KS = D / 32, DT = D / 16;
     // K and V of a tile in registers at once, where they leave room for two waves per SIMD.
-    constexpr bool BOTH = D <= 128 || Q8;
+    constexpr bool BOTH = D < 128 || Q8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     const ItemRows x = item_rows<OWN>(a, item, 16, lane);
     if (x.r0 >= x.r1) return;
@@ -568,10 +606,8 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs& a, uint4* lds, int i
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                float y[8];
-                t.k_values(u, s, fk, y);
                 f16x8 kh, kl;
-                split8(y, kh, kl);
+                t.k_split(u, s, fk, kh, kl);
                 st[0][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[s], st[0][u], 0, 0, 0);
                 st[0][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[s], st[0][u], 0, 0, 0);
                 st[0][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[s], st[0][u], 0, 0, 0);
@@ -620,10 +656,8 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs& a, uint4* lds, int i
         const float fv = pk::pow2i(-ev);
 #pragma unroll
         for (int tt = 0; tt < DT; ++tt) {
-            float y[8];
-            t.v_values(tt, fv, y);
             f16x8 vh, vl;
-            split8(y, vh, vl);
+            t.v_split(tt, fv, vh, vl);
             o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[0], o[tt], 0, 0, 0);
             o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[0], o[tt], 0, 0, 0);
             o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[0], o[tt], 0, 0, 0);
@@ -776,7 +810,7 @@ struct TilePart {
                 x = fmaxf(x, fabsf(k[i][0][2]) * 128.0f);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x = fmaxf(x, fabsf(k[i][e >> 2][e & 3]));
+                for (int e = 0; e < 8; e += 2) x = max_abs(x, k[i][e >> 2][e & 3], k[i][e >> 2][(e & 3) + 1]);
             }
         }
         return x;
@@ -792,7 +826,7 @@ struct TilePart {
                     x = fmaxf(x, fabsf(v[i][j][1]) * 128.0f);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x = fmaxf(x, fabsf(v[i][j][e]));
+                    for (int e = 0; e < 4; e += 2) x = max_abs(x, v[i][j][e], v[i][j][e + 1]);
                 }
             }
         }
@@ -808,10 +842,9 @@ struct TilePart {
             if (NK % 4 != 0 && q >= NK) break;
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x[e] = Q8 ? quant(k[i][0][e >> 2], e & 3) * (k[i][0][2] * fk) : k[i][e >> 2][e & 3] * fk;
+            for (int e = 0; e < 8; ++e) x[e] = Q8 ? quant(k[i][0][e >> 2], e & 3) : k[i][e >> 2][e & 3];
             f16x8 hi, lo;
-            split8(x, hi, lo);
+            split8(x, Q8 ? k[i][0][2] * fk : fk, hi, lo);
             lds[(2 * q + 0) * 64 + lane] = __builtin_bit_cast(uint4, hi);
             lds[(2 * q + 1) * 64 + lane] = __builtin_bit_cast(uint4, lo);
         }
@@ -824,14 +857,16 @@ struct TilePart {
 #pragma unroll
             for (int t = 0; t < 4; t += 2) {   // columns t and t + 1
                 if (REM && c >= NC && t > 0) break;
-                float x[8];
+                float x[8], y[8];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int w = 0; w < 2; ++w)
-                        x[4 * w + j] = Q8 ? quant(v[i][j][0], t + w) * (v[i][j][1] * fv) : v[i][j][t + w] * fv;
+                    for (int w = 0; w < 2; ++w) {
+                        x[4 * w + j] = Q8 ? quant(v[i][j][0], t + w) : v[i][j][t + w];
+                        y[4 * w + j] = Q8 ? v[i][j][1] * fv : fv;
+                    }
                 f16x8 hi, lo;
-                split8(x, hi, lo);
+                split8(x, y, hi, lo);
                 const uint4 uh = __builtin_bit_cast(uint4, hi), ul = __builtin_bit_cast(uint4, lo);
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
@@ -845,13 +880,16 @@ struct TilePart {
 };
 
 // 64*MT query rows, 16*MT a wave, against a split of the prefix, or (OWN) of one sequence's own rows.
+// Two tiles in LDS (one at head_dim 256, whose two would leave room for one workgroup a CU): while the
+// waves multiply tile i, they hold tile i + 2 in flight and have stored i + 1.
 template <int D, int MT, bool Q8, bool OWN>
 __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int item, int h, int split) {
     using T = TilePart<D, Q8>;
-    constexpr int KS = D / 32, DT = D / 16, NK = T::NK;
-    __shared__ int s_range[2][kAttnWaves];
-    __shared__ float s_max[2][kAttnWaves];
-    __shared__ unsigned s_bad[kAttnWaves];
+    constexpr int KS = D / 32, DT = D / 16, NK = T::NK, kTileU4 = T::kBytes / 16;
+    constexpr bool TWO = wide_tiles(D) == 2;
+    __shared__ int s_range[4][kAttnWaves];
+    __shared__ float s_max[2][2][kAttnWaves];
+    __shared__ unsigned s_bad[2][kAttnWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
     const ItemRows x = item_rows<OWN>(a, item, 64 * MT, lane);
     if (x.r0 >= x.r1) return;
@@ -882,16 +920,19 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
     if (lane == 0) {
         s_range[0][wave] = lo_any;
         s_range[1][wave] = hi_any;
+        s_range[2][wave] = lo_all;
+        s_range[3][wave] = hi_all;
     }
     __syncthreads();
-    int lo = s_range[0][0], hi = s_range[1][0];
+    // Of all waves: the rows that some query attends, and those that every query does.
+    auto all_waves = [&](int which, bool most) {
+        int y = s_range[which][0];
 #pragma unroll
-    for (int w = 1; w < kAttnWaves; ++w) {
-        lo = min(lo, s_range[0][w]);
-        hi = max(hi, s_range[1][w]);
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    hi = __builtin_amdgcn_readfirstlane(hi);
+        for (int w = 1; w < kAttnWaves; ++w) y = most ? max(y, s_range[which][w]) : min(y, s_range[which][w]);
+        return __builtin_amdgcn_readfirstlane(y);
+    };
+    int lo = all_waves(0, false), hi = all_waves(1, true);
+    const int lo_every = all_waves(2, true), hi_every = all_waves(3, false);
     if constexpr (OWN) lo = max(a.prefix, lo);
     else hi = min(a.prefix, hi);
     int t_lo, t_hi;
@@ -901,51 +942,62 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
     const int rmask = (1 << a.pool.shift) - 1;
     auto entry = [&](int tile, int u) { return x.blk[min((tile * kTile + 16 * u) >> a.pool.shift, a.width - 1)]; };
     auto in_pool = [&](int e) { return paged_page_ok(e, a.pool.n_pages); };
+    // The loaded tile t (its pages c0, c1), the next one's table entries n0, n1.
     T t;
     int n0 = 0, n1 = 0, c0 = 0, c1 = 0;
-    auto load = [&](int at) {
-        t.load(a.pool, in_pool(c0) ? c0 : 0, in_pool(c1) ? c1 : 0, h, at * kTile & rmask, (at * kTile + 16) & rmask, wave, n, g);
-    };
-    if (t_lo < t_hi) {
-        const int e0 = entry(t_lo, 0), e1 = entry(t_lo, 1);
-        n0 = entry(t_lo + 1, 0);
-        n1 = entry(t_lo + 1, 1);
-        c0 = __builtin_amdgcn_readfirstlane(e0);
-        c1 = __builtin_amdgcn_readfirstlane(e1);
-        load(t_lo);
-    }
-    const f16x8* op = reinterpret_cast<const f16x8*>(lds);
-    for (int tile = t_lo; tile < t_hi; ++tile) {
-        const int k0 = tile * kTile;
-        const bool there0 = in_pool(c0), there1 = in_pool(c1);
-        auto held = [&](int row) { return (row < 16 ? there0 : there1) && k0 + row >= lo && k0 + row < hi; };
-        const bool whole = k0 >= lo && k0 + kTile <= hi && there0 && there1;
-        // Whether every wave's queries attend all of the tile is the wave's own matter (plain, below);
-        // a value that is not finite has to be taken out wherever some query does not attend its row.
-        unsigned bad = t.clean(held, wave, n, g);
-        const float mk = wave_max(t.max_k(wave)), mv = wave_max(t.max_v(wave));
-        bad = __ballot(bad) != 0 ? wave_or(bad) : 0u;
-        if (lane == 0) {
-            s_max[0][wave] = mk;
-            s_max[1][wave] = mv;
-            s_bad[wave] = bad;
-        }
-        __syncthreads();   // and the last reads of the tile before
-        const float ak = fmaxf(fmaxf(s_max[0][0], s_max[0][1]), fmaxf(s_max[0][2], s_max[0][3]));
-        const float av = fmaxf(fmaxf(s_max[1][0], s_max[1][1]), fmaxf(s_max[1][2], s_max[1][3]));
-        const unsigned poison = __builtin_amdgcn_readfirstlane(s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]);
-        const int ek = __builtin_amdgcn_readfirstlane(fit_exp(ak));
-        const float fe = raise_exp(ev, __builtin_amdgcn_readfirstlane(fit_exp(av)));
-        t.store(lds, pk::pow2i(-ek), pk::pow2i(-ev), wave, lane);
+    auto load = [&](int tile) {
         c0 = __builtin_amdgcn_readfirstlane(n0);
         c1 = __builtin_amdgcn_readfirstlane(n1);
-        if (tile + 1 < t_hi) {
-            n0 = entry(tile + 2, 0);
-            n1 = entry(tile + 2, 1);
-            load(tile + 1);
+        n0 = entry(tile + 1, 0);
+        n1 = entry(tile + 1, 1);
+        t.load(a.pool, in_pool(c0) ? c0 : 0, in_pool(c1) ? c1 : 0, h, tile * kTile & rmask, (tile * kTile + 16) & rmask, wave, n, g);
+    };
+    // The loaded tile's largest values, for the exponents; and where some query does not attend all of
+    // it, or a value is infinite, what is not to be multiplied is taken out.
+    auto inspect = [&](int tile) {
+        const int k0 = tile * kTile, slot = (tile - t_lo) & 1;
+        const bool there0 = in_pool(c0), there1 = in_pool(c1);
+        unsigned bad = 0;
+        float mk = wave_max(t.max_k(wave)), mv = wave_max(t.max_v(wave));
+        const bool every = k0 >= max(lo, lo_every) && k0 + kTile <= min(hi, hi_every) && there0 && there1;
+        if (!every || !finite_bits(__float_as_uint(mk)) || !finite_bits(__float_as_uint(mv))) {
+            auto held = [&](int row) { return (row < 16 ? there0 : there1) && k0 + row >= lo && k0 + row < hi; };
+            bad = t.clean(held, wave, n, g);
+            bad = __ballot(bad) != 0 ? wave_or(bad) : 0u;
+            mk = wave_max(t.max_k(wave));
+            mv = wave_max(t.max_v(wave));
         }
-        __syncthreads();
-        if (rw >= x.r1) continue;   // no rows of its own: only the loads are its work
+        if (lane == 0) {
+            s_max[slot][0][wave] = mk;
+            s_max[slot][1][wave] = mv;
+            s_bad[slot][wave] = bad;
+        }
+    };
+    // The inspected tile to LDS, and what its multiplication has to know.
+    struct Stored {
+        int ek;
+        float fe;             // factor of the outputs that V's exponent brings
+        unsigned poison;      // rows (bit = row of the tile) that hold a value that is not finite
+        bool there0, there1;
+    };
+    auto store = [&](int tile) {
+        const int slot = (tile - t_lo) & 1;
+        const float(&y)[2][kAttnWaves] = s_max[slot];
+        const float ak = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3]));
+        const float av = fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3]));
+        Stored r;
+        r.poison = __builtin_amdgcn_readfirstlane(s_bad[slot][0] | s_bad[slot][1] | s_bad[slot][2] | s_bad[slot][3]);
+        r.ek = __builtin_amdgcn_readfirstlane(fit_exp(ak));
+        r.fe = raise_exp(ev, __builtin_amdgcn_readfirstlane(fit_exp(av)));
+        r.there0 = in_pool(c0);
+        r.there1 = in_pool(c1);
+        t.store(lds + (TWO ? slot * kTileU4 : 0), pk::pow2i(-r.ek), pk::pow2i(-ev), wave, lane);
+        return r;
+    };
+    auto multiply = [&](int tile, const Stored& now) {
+        if (rw >= x.r1) return;   // no rows of its own: only the loads are its work
+        const int k0 = tile * kTile;
+        const f16x8* op = reinterpret_cast<const f16x8*>(lds + (TWO ? ((tile - t_lo) & 1) * kTileU4 : 0));
         floatx4 st[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) st[mt][0] = st[mt][1] = floatx4{0, 0, 0, 0};
@@ -960,14 +1012,16 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
                 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[mt][q % KS], c, 0, 0, 0);
             }
         }
-        const bool plain = whole && k0 >= lo_all && k0 + kTile <= hi_all;
+        auto held = [&](int row) { return (row < 16 ? now.there0 : now.there1) && k0 + row >= lo && k0 + row < hi; };
         auto attended = [&](int mt, int row) { return held(row) && k0 + row >= first[mt] && k0 + row <= pos[mt]; };
+        const bool plain = k0 >= max(lo, lo_all) && k0 + kTile <= min(hi, hi_all) && now.there0 && now.there1;
         f16x8 ph[MT], pl[MT];
-        const bool rescale = tile_softmax<MT>(a, st, pk::pow2i(ek), fq, m, l, alpha, ph, pl, !plain || poison, poison, g, attended);
-        if (rescale || fe != 1.0f) {
+        const bool rescale =
+            tile_softmax<MT>(a, st, pk::pow2i(now.ek), fq, m, l, alpha, ph, pl, !plain || now.poison, now.poison, g, attended);
+        if (rescale || now.fe != 1.0f) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const float f = alpha[mt] * fe;
+                const float f = alpha[mt] * now.fe;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[mt][d] = o[mt][d] * f;
             }
@@ -981,6 +1035,42 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
                 o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[mt], o[mt][tt], 0, 0, 0);
                 o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[mt], o[mt][tt], 0, 0, 0);
             }
+        }
+    };
+    if (t_lo < t_hi) {
+        n0 = entry(t_lo, 0);
+        n1 = entry(t_lo, 1);
+        load(t_lo);
+        inspect(t_lo);
+    }
+    __syncthreads();
+    if constexpr (TWO) {
+        Stored now{};
+        if (t_lo < t_hi) {
+            now = store(t_lo);
+            if (t_lo + 1 < t_hi) {
+                load(t_lo + 1);
+                inspect(t_lo + 1);
+            }
+        }
+        __syncthreads();
+        for (int tile = t_lo; tile < t_hi; ++tile) {
+            Stored next = now;
+            if (tile + 1 < t_hi) next = store(tile + 1);   // into the tile that was multiplied before the barrier
+            if (tile + 2 < t_hi) load(tile + 2);
+            multiply(tile, now);
+            if (tile + 2 < t_hi) inspect(tile + 2);
+            now = next;
+            __syncthreads();
+        }
+    } else {
+        for (int tile = t_lo; tile < t_hi; ++tile) {
+            const Stored now = store(tile);
+            if (tile + 1 < t_hi) load(tile + 1);
+            __syncthreads();
+            multiply(tile, now);
+            if (tile + 1 < t_hi) inspect(tile + 1);
+            __syncthreads();
         }
     }
     const float f = ev < -500 ? 0.0f : pk::pow2i(ev);
