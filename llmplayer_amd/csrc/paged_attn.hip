@@ -28,8 +28,10 @@ hipError_t launch(pg::AttnArgs a, hipStream_t st) {
 // The pairs that paged_plan gives: an item of all tokens has at least the rows of one sequence's.
 template <int D, bool Q8>
 hipError_t launch_rows(const pg::AttnArgs& a, int wp, int wo, hipStream_t st) {
-    if (wp == 0 && wo == 0) return launch<D, 0, 0, Q8>(a, st);
-    if (wp == 1 && wo == 0) return launch<D, 1, 0, Q8>(a, st);
+    if constexpr (paged_narrow(D)) {
+        if (wp == 0 && wo == 0) return launch<D, 0, 0, Q8>(a, st);
+        if (wp == 1 && wo == 0) return launch<D, 1, 0, Q8>(a, st);
+    }
     if (wp == 1 && wo == 1) return launch<D, 1, 1, Q8>(a, st);
     if constexpr (paged_wide_max(D) == 2) {
         if (wp == 2 && wo == 0) return launch<D, 2, 0, Q8>(a, st);

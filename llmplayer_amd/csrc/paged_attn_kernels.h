@@ -95,10 +95,14 @@ __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo
 template <int D, bool Q8>
 struct Tile;
 
-// Address of row r of a page of plane p (elements of `unit` values per row).
+// Address of row `row` (alike in all lanes) of KV head h of a page, rows of `unit` bytes; a lane adds
+// its own part as a 32-bit offset, so that one scalar base serves all of its loads.
+__device__ __forceinline__ const char* page_rows(const void* p, const PoolPlanes& pool, int page, int h, int row, int unit) {
+    return static_cast<const char*>(p) + ((((long long)page * pool.n_kv_heads + h) << pool.shift) + row) * unit;
+}
 template <class T>
-__device__ __forceinline__ const T* page_row(const void* p, const PoolPlanes& pool, int page, int h, int row, int unit) {
-    return static_cast<const T*>(p) + ((((long long)page * pool.n_kv_heads + h) << pool.shift) + row) * unit;
+__device__ __forceinline__ T at(const char* base, unsigned offset) {
+    return *reinterpret_cast<const T*>(base + offset);
 }
 
 __device__ __forceinline__ bool finite_bits(unsigned b) { return (b & 0x7F800000u) != 0x7F800000u; }
@@ -113,22 +117,24 @@ struct Tile<D, false> {
     __device__ __forceinline__ void load_k(const PoolPlanes& p, int page0, int page1, int h, int r0, int r1, int n, int g) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const float* x = page_row<float>(p.k, p, u ? page1 : page0, h, (u ? r1 : r0) + n, D) + 8 * g;
+            const char* b = page_rows(p.k, p, u ? page1 : page0, h, u ? r1 : r0, 4 * D);
+            const unsigned lane = (unsigned)(4 * D * n + 32 * g);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                k[u][s][0] = *reinterpret_cast<const floatx4*>(x + 32 * s);
-                k[u][s][1] = *reinterpret_cast<const floatx4*>(x + 32 * s + 4);
+                k[u][s][0] = at<floatx4>(b, lane + 128 * s);
+                k[u][s][1] = at<floatx4>(b, lane + 128 * s + 16);
             }
         }
     }
     __device__ __forceinline__ void load_v(const PoolPlanes& p, int page0, int page1, int h, int r0, int r1, int n, int g) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float* x = page_row<float>(p.v, p, j < 4 ? page0 : page1, h, (j < 4 ? r0 : r1) + 4 * g + (j & 3), D);
+            const char* b = page_rows(p.v, p, j < 4 ? page0 : page1, h, j < 4 ? r0 : r1, 4 * D);
+            const unsigned row = (unsigned)(4 * D * 4 * g) + 4 * D * (j & 3);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) v[j][c] = *reinterpret_cast<const floatx4*>(x + 64 * c + 4 * n);
+            for (int c = 0; c < NC; ++c) v[j][c] = at<floatx4>(b, row + 16 * n + 256 * c);
             if constexpr (REM) {
-                const float2 w = *reinterpret_cast<const float2*>(x + 64 * NC + 2 * n);
+                const float2 w = at<float2>(b, row + 8 * n + 256 * NC);
                 vr[j][0] = w.x;
                 vr[j][1] = w.y;
             }
@@ -227,29 +233,30 @@ struct Tile<D, true> {
     __device__ __forceinline__ void load_k(const PoolPlanes& p, int page0, int page1, int h, int r0, int r1, int n, int g) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const signed char* x = page_row<signed char>(p.k, p, u ? page1 : page0, h, (u ? r1 : r0) + n, D) + 8 * g;
-            const float* sc = page_row<float>(p.ks, p, u ? page1 : page0, h, (u ? r1 : r0) + n, KS);
+            const char* b = page_rows(p.k, p, u ? page1 : page0, h, u ? r1 : r0, D);
+            const char* sc = page_rows(p.ks, p, u ? page1 : page0, h, u ? r1 : r0, 4 * KS);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                k[u][s] = *reinterpret_cast<const uint2*>(x + 32 * s);
-                ks[u][s] = sc[s];
+                k[u][s] = at<uint2>(b, (unsigned)(D * n + 8 * g) + 32 * s);
+                ks[u][s] = at<float>(sc, (unsigned)(4 * KS * n) + 4 * s);
             }
         }
     }
     __device__ __forceinline__ void load_v(const PoolPlanes& p, int page0, int page1, int h, int r0, int r1, int n, int g) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int page = j < 4 ? page0 : page1, row = (j < 4 ? r0 : r1) + 4 * g + (j & 3);
-            const signed char* x = page_row<signed char>(p.v, p, page, h, row, D);
-            const float* sc = page_row<float>(p.vs, p, page, h, row, KS);
+            const int page = j < 4 ? page0 : page1, r = j < 4 ? r0 : r1;
+            const char* b = page_rows(p.v, p, page, h, r, D);
+            const char* sc = page_rows(p.vs, p, page, h, r, 4 * KS);
+            const unsigned row = (unsigned)(4 * g) + (j & 3);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                v[j][c] = *reinterpret_cast<const unsigned*>(x + 64 * c + 4 * n);
-                vs[j][c] = sc[2 * c + (n >> 3)];
+                v[j][c] = at<unsigned>(b, row * D + 4 * n + 64 * c);
+                vs[j][c] = at<float>(sc, row * (4 * KS) + 4 * (n >> 3) + 8 * c);
             }
             if constexpr (REM) {
-                v[j][NC] = *reinterpret_cast<const unsigned short*>(x + 64 * NC + 2 * n);
-                vs[j][NC] = sc[2 * NC];
+                v[j][NC] = at<unsigned short>(b, row * D + 2 * n + 64 * NC);
+                vs[j][NC] = at<float>(sc, row * (4 * KS) + 8 * NC);
             }
         }
     }
@@ -310,15 +317,28 @@ struct Tile<D, true> {
     }
 };
 
-// Largest value over the wave.
+// Largest of non-negative floats (their bits) over the wave, and of two packed 16-bit halves each.
+template <class Max>
+__device__ __forceinline__ unsigned wave_reduce(unsigned x, const Max& max_of) {
+    auto step = [&](auto ctrl) {
+        x = max_of(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xF, 0xF, false));
+    };
+    step(std::integral_constant<int, dk::kDppQuadXor1>{});
+    step(std::integral_constant<int, dk::kDppQuadXor2>{});
+    step(std::integral_constant<int, dk::kDppRowHalfMirror>{});
+    step(std::integral_constant<int, dk::kDppRowMirror>{});
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max_of((unsigned)a[0], (unsigned)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = max_of((unsigned)b[0], (unsigned)b[1]);
+    return __builtin_amdgcn_readfirstlane(x);
+}
 __device__ __forceinline__ float wave_max(float x) {
-    x = fmaxf(x, dk::dpp<dk::kDppQuadXor1>(x));
-    x = fmaxf(x, dk::dpp<dk::kDppQuadXor2>(x));
-    x = dk::lane_step<4, true>(x);
-    x = dk::lane_step<8, true>(x);
-    x = dk::lane_step<16, true>(x);
-    x = dk::lane_step<32, true>(x);
-    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+    return __uint_as_float(wave_reduce(__float_as_uint(x), [](unsigned a, unsigned b) { return max(a, b); }));
+}
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned max_halves(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 // Exponent e with max * 2^-e in [2^13, 2^14) (0 for 0; clamped so that 2^e and 2^-e are normal).
 __device__ __forceinline__ int fit_exp(float mx) {
@@ -336,13 +356,6 @@ __device__ __forceinline__ unsigned wave_or(unsigned x) {
 // rows 4g + i and 16 + 4g + i.
 __device__ __forceinline__ unsigned tile_rows(unsigned bk, unsigned bv, int n, int g) {
     return wave_or((bk & 1u) << n | (bk >> 1) << (16 + n) | (bv & 15u) << (4 * g) | (bv >> 4) << (16 + 4 * g));
-}
-
-// Tiles that attn_wide holds, and the dynamic LDS: these, or the waves' states that attn_narrow joins.
-constexpr int wide_tiles(int D) { return D <= 128 ? 2 : 1; }
-template <int D>
-constexpr size_t attn_lds(int wide) {
-    return wide ? (size_t)wide_tiles(D) * (D / 16 + D / 16) * 2 * 64 * 16 : 2 * (size_t)(D / 4 + 2) * 64 * 4;
 }
 
 // The sequence of work item `item` of an own-rows launch (paged_item_base).
@@ -440,10 +453,11 @@ __device__ __forceinline__ void split_tiles(const AttnArgs& a, int row_lo, int r
 // split of p = 2^(s - m).  The maxima are only raised where a score passes the present one by 2^12 or more
 // (p stays below 2^12, which fp16 holds), so that most tiles leave o as it is: true where o has to be
 // multiplied by alpha.  poison: rows of the tile that make a NaN of what attends them.
-template <int MT, class Attended>
-__device__ __forceinline__ bool tile_softmax(const AttnArgs& a, floatx4 (&st)[MT][2], float fkr, const float (&fq)[MT],
-                                             float (&m)[MT], float (&l)[MT], float (&alpha)[MT], f16x8 (&ph)[MT],
-                                             f16x8 (&pl)[MT], bool masked, unsigned poison, int g, const Attended& attended) {
+template <int MT, int NU, class Attended>
+__device__ __forceinline__ bool tile_softmax(const AttnArgs& a, floatx4 (&st)[MT][NU], float fkr, const float (&fq)[MT],
+                                             float (&m)[MT], float (&l)[MT], float (&alpha)[MT], f16x8 (&ph)[MT][NU / 2],
+                                             f16x8 (&pl)[MT][NU / 2], bool masked, unsigned long long poison, int g,
+                                             const Attended& attended) {
     float fs[MT], mx[MT];
     bool up = false;
 #pragma unroll
@@ -452,14 +466,14 @@ __device__ __forceinline__ bool tile_softmax(const AttnArgs& a, floatx4 (&st)[MT
         if (a.softcap > 0.0f) {
             const float isc = a.inv_softcap * fs[mt];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) st[mt][u][i] = a.softcap_log2e * tanhf(st[mt][u][i] * isc);
             fs[mt] = 1.0f;
         }
         if (masked) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = 16 * u + 4 * g + i;
@@ -469,7 +483,7 @@ __device__ __forceinline__ bool tile_softmax(const AttnArgs& a, floatx4 (&st)[MT
         }
         float x = kNegBig;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) x = fmaxf(x, st[mt][u][i]);
         x = dk::lane_step<16, true>(x);
@@ -483,16 +497,18 @@ __device__ __forceinline__ bool tile_softmax(const AttnArgs& a, floatx4 (&st)[MT
         const float mn = rescale ? fmaxf(m[mt], mx[mt] - kPShift) : m[mt];
         alpha[mt] = dk::fast_exp2(m[mt] - mn);
         m[mt] = mn;
-        float p[8], sum = 0.0f;
+        float sum = 0.0f;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int w = 0; w < NU / 2; ++w) {
+            float p[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                p[4 * u + i] = dk::fast_exp2(__builtin_fmaf(st[mt][u][i], fs[mt], -mn));
-                sum += p[4 * u + i];
+            for (int i = 0; i < 8; ++i) {
+                p[i] = dk::fast_exp2(__builtin_fmaf(st[mt][2 * w + (i >> 2)][i & 3], fs[mt], -mn));
+                sum += p[i];
             }
+            split8(p, ph[mt][w], pl[mt][w]);
+        }
         l[mt] = __builtin_fmaf(l[mt], alpha[mt], sum);
-        split8(p, ph[mt], pl[mt]);
     }
     return rescale;
 }
@@ -621,8 +637,8 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs& a, uint4* lds, int i
             n1 = entry(next + kAttnWaves, 1);
             if constexpr (BOTH) load_k(next);
         }
-        f16x8 ph[1], pl[1];
-        bool rescale = tile_softmax<1>(a, st, fkr, fq, m, l, alpha, ph, pl, !plain || poison, poison, g, attended);
+        f16x8 ph[1][1], pl[1][1];
+        const bool rescale = tile_softmax<1, 2>(a, st, fkr, fq, m, l, alpha, ph, pl, !plain || poison, poison, g, attended);
         unsigned bv = 0;
         if (!plain) {
             unsigned ok = 0;
@@ -642,7 +658,7 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs& a, uint4* lds, int i
             for (int j = 0; j < 8; ++j) {
                 const int row = 16 * (j >> 2) + 4 * g + (j & 3);
                 if ((poison >> row & 1) && attended(0, row)) {
-                    ph[0][j] = (_Float16)__builtin_nanf("");
+                    ph[0][0][j] = (_Float16)__builtin_nanf("");
                     l[0] = __builtin_nanf("");
                 }
             }
@@ -658,9 +674,9 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs& a, uint4* lds, int i
         for (int tt = 0; tt < DT; ++tt) {
             f16x8 vh, vl;
             t.v_split(tt, fv, vh, vl);
-            o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[0], o[tt], 0, 0, 0);
-            o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[0], o[tt], 0, 0, 0);
-            o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[0], o[tt], 0, 0, 0);
+            o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[0][0], o[tt], 0, 0, 0);
+            o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[0][0], o[tt], 0, 0, 0);
+            o[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[0][0], o[tt], 0, 0, 0);
         }
         if (next < t_hi) {
             if constexpr (BOTH) load_v(next, c0, c1);
@@ -707,53 +723,71 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs& a, uint4* lds, int i
 }
 
 // ---- a tile shared by four waves ---------------------------------------------------------------
-// In LDS: K as [2 half tiles x D/32 steps][hi, lo][lane] and V as [D/16 output tiles][hi, lo][lane], 16
-// bytes a lane, exactly the operands: every read is one conflict-free b128.  A wave loads, cleans and
-// splits the K operands p = wave, wave + 4, ... and the V units (64 dims, half tile) likewise; a unit's
-// lane holds 4 rows of 4 dims, 8 bytes of four operands.
+// Rows of it: 64 at head_dim 64, 32 above (the same bytes).  In LDS: K as [16-row parts x D/32 steps][hi,
+// lo][lane] and V as [32-row groups x D/16 output tiles][hi, lo][lane], 16 bytes a lane, exactly the
+// operands: every read is one conflict-free b128.  A wave loads, cleans and splits the K operands
+// p = wave, wave + 4, ... and the V units (64 dims, 16-row part) likewise; a unit's lane holds 4 rows of 4
+// dims, 8 bytes of four operands.
+constexpr int wide_rows(int D) { return D == 64 ? 64 : 32; }
+constexpr int wide_tiles(int D) { return D <= 128 ? 2 : 1; }
+
 template <int D, bool Q8>
 struct TilePart {
-    static constexpr int KS = D / 32, NC = D / 64, REM = D % 64 / 32;
-    static constexpr int NK = 2 * KS, NV = 2 * (NC + REM);
+    static constexpr int KS = D / 32, NC = D / 64, REM = D % 64 / 32, DT = D / 16, NU = wide_rows(D) / 16;
+    static constexpr int NK = NU * KS, NV = NU * (NC + REM);
     static constexpr int KP = (NK + 3) / 4, VP = (NV + 3) / 4;
-    static constexpr int kBytes = (NK + D / 16) * 2 * 64 * 16;
+    static constexpr int kBytes = (NK + NU / 2 * DT) * 2 * 64 * 16;
     floatx4 k[KP][2];      // Q8: 8 quants in the first two words, the scale in the third
     floatx4 v[VP][4];      // Q8: 4 quants and their scale
 
-    __device__ __forceinline__ void load(const PoolPlanes& p, int page0, int page1, int h, int r0, int r1, int wave, int n, int g) {
+    // The 16-row part of K operand q and of V unit q, and its 64 dims.
+    static __device__ __forceinline__ int k_part(int q) { return q / KS; }
+    static __device__ __forceinline__ int v_part(int q) { return q % NU; }
+    static __device__ __forceinline__ int v_dims(int q) { return q / NU; }
+
+    // The pages of the wave's parts (kp, vp), and row(u): the first row in its page of 16-row part u.
+    template <class Row>
+    __device__ __forceinline__ void load(const PoolPlanes& p, const int (&kp)[KP], const int (&vp)[VP], const Row& row, int h,
+                                         int wave, int n, int g) {
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             const int q = wave + 4 * i;
             if (NK % 4 != 0 && q >= NK) break;
-            const int u = q / KS, s = q % KS, page = u ? page1 : page0, row = (u ? r1 : r0) + n;
+            const int u = k_part(q), s = q % KS;
             if constexpr (Q8) {
-                const uint2 w = *reinterpret_cast<const uint2*>(page_row<signed char>(p.k, p, page, h, row, D) + 32 * s + 8 * g);
-                k[i][0] = floatx4{__uint_as_float(w.x), __uint_as_float(w.y), page_row<float>(p.ks, p, page, h, row, KS)[s], 0};
+                const uint2 w = at<uint2>(page_rows(p.k, p, kp[i], h, row(u), D) + 32 * s, D * n + 8 * g);
+                k[i][0] = floatx4{__uint_as_float(w.x), __uint_as_float(w.y),
+                                  at<float>(page_rows(p.ks, p, kp[i], h, row(u), 4 * KS) + 4 * s, 4 * KS * n), 0};
             } else {
-                const float* x = page_row<float>(p.k, p, page, h, row, D) + 32 * s + 8 * g;
-                k[i][0] = *reinterpret_cast<const floatx4*>(x);
-                k[i][1] = *reinterpret_cast<const floatx4*>(x + 4);
+                const char* b = page_rows(p.k, p, kp[i], h, row(u), 4 * D) + 128 * s;
+                k[i][0] = at<floatx4>(b, 4 * D * n + 32 * g);
+                k[i][1] = at<floatx4>(b, 4 * D * n + 32 * g + 16);
             }
         }
 #pragma unroll
         for (int i = 0; i < VP; ++i) {
             const int q = wave + 4 * i;
             if (NV % 4 != 0 && q >= NV) break;
-            const int c = q >> 1, page = q & 1 ? page1 : page0, row = (q & 1 ? r1 : r0) + 4 * g;
+            const int u = v_part(q), c = v_dims(q);
+            if constexpr (Q8) {
+                const char* b = page_rows(p.v, p, vp[i], h, row(u), D) + 64 * c;
+                const char* sc = page_rows(p.vs, p, vp[i], h, row(u), 4 * KS) + 8 * c;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (Q8) {
-                    const signed char* x = page_row<signed char>(p.v, p, page, h, row + j, D) + 64 * c;
-                    const unsigned w = c < NC ? *reinterpret_cast<const unsigned*>(x + 4 * n)
-                                              : *reinterpret_cast<const unsigned short*>(x + 2 * n);
-                    const int b = c < NC ? 2 * c + (n >> 3) : 2 * NC;
-                    v[i][j] = floatx4{__uint_as_float(w), page_row<float>(p.vs, p, page, h, row + j, KS)[b], 0, 0};
-                } else {
-                    const float* x = page_row<float>(p.v, p, page, h, row + j, D) + 64 * c;
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned r = 4 * g + j;
+                    const bool full = REM == 0 || c < NC;
+                    const unsigned w = full ? at<unsigned>(b, D * r + 4 * n) : at<unsigned short>(b, D * r + 2 * n);
+                    v[i][j] = floatx4{__uint_as_float(w), at<float>(sc, 4 * KS * r + (full ? 4 * (n >> 3) : 0)), 0, 0};
+                }
+            } else {
+                const char* b = page_rows(p.v, p, vp[i], h, row(u), 4 * D) + 256 * c;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned r = 4 * D * (4 * g + j);
                     if (REM == 0 || c < NC) {
-                        v[i][j] = *reinterpret_cast<const floatx4*>(x + 4 * n);
+                        v[i][j] = at<floatx4>(b, r + 16 * n);
                     } else {
-                        const float2 w = *reinterpret_cast<const float2*>(x + 2 * n);
+                        const float2 w = at<float2>(b, r + 8 * n);
                         v[i][j] = floatx4{w.x, w.y, 0, 0};
                     }
                 }
@@ -763,14 +797,14 @@ struct TilePart {
     // Takes out what no row holds (held(row) false) and what is not finite; returns the rows (bit = row
     // of the tile) of the lane's share that held such a value.
     template <class Held>
-    __device__ __forceinline__ unsigned clean(const Held& held, int wave, int n, int g) {
+    __device__ __forceinline__ unsigned long long clean(const Held& held, int wave, int n, int g) {
         using C = Tile<D, false>;
-        unsigned bad = 0;
+        unsigned long long bad = 0;
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             const int q = wave + 4 * i;
             if (NK % 4 != 0 && q >= NK) break;
-            const int row = 16 * (q / KS) + n;
+            const int row = 16 * k_part(q) + n;
             const unsigned keep = 0u - (unsigned)held(row);
             unsigned worst = 0;
             if constexpr (Q8) {
@@ -779,7 +813,7 @@ struct TilePart {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) k[i][e >> 2][e & 3] = C::clean(k[i][e >> 2][e & 3], keep, worst);
             }
-            bad |= (unsigned)(worst >= 0x7F800000u) << row;
+            bad |= (unsigned long long)(worst >= 0x7F800000u) << row;
         }
 #pragma unroll
         for (int i = 0; i < VP; ++i) {
@@ -787,7 +821,7 @@ struct TilePart {
             if (NV % 4 != 0 && q >= NV) break;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int row = 16 * (q & 1) + 4 * g + j;
+                const int row = 16 * v_part(q) + 4 * g + j;
                 const unsigned keep = 0u - (unsigned)held(row);
                 unsigned worst = 0;
                 if constexpr (Q8) {
@@ -796,41 +830,38 @@ struct TilePart {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[i][j][e] = C::clean(v[i][j][e], keep, worst);
                 }
-                bad |= (unsigned)(worst >= 0x7F800000u) << row;
+                bad |= (unsigned long long)(worst >= 0x7F800000u) << row;
             }
         }
         return bad;
     }
-    __device__ __forceinline__ float max_k(int wave) const {
-        float x = 0.0f;
+    // The wave's largest magnitudes: bits 16-31 of K's in the low half, of V's in the high half.
+    __device__ __forceinline__ unsigned largest(int wave) const {
+        float x = 0.0f, y = 0.0f;
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             if (NK % 4 != 0 && wave + 4 * i >= NK) break;
             if constexpr (Q8) {
-                x = fmaxf(x, fabsf(k[i][0][2]) * 128.0f);
+                x = max_abs(x, k[i][0][2], k[i][0][2]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) x = max_abs(x, k[i][e >> 2][e & 3], k[i][e >> 2][(e & 3) + 1]);
             }
         }
-        return x;
-    }
-    __device__ __forceinline__ float max_v(int wave) const {
-        float x = 0.0f;
 #pragma unroll
         for (int i = 0; i < VP; ++i) {
             if (NV % 4 != 0 && wave + 4 * i >= NV) break;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (Q8) {
-                    x = fmaxf(x, fabsf(v[i][j][1]) * 128.0f);
+                    y = max_abs(y, v[i][j][1], v[i][j][1]);
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) x = max_abs(x, v[i][j][e], v[i][j][e + 1]);
+                    y = max_abs(y, v[i][j][0], v[i][j][1]);
+                    y = max_abs(y, v[i][j][2], v[i][j][3]);
                 }
             }
         }
-        return x;
+        return wave_reduce(__builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u), max_halves);
     }
     static __device__ __forceinline__ float quant(float word, int byte) {
         return (float)(signed char)(__float_as_uint(word) >> (8 * byte) & 0xFF);
@@ -853,7 +884,7 @@ struct TilePart {
         for (int i = 0; i < VP; ++i) {
             const int q = wave + 4 * i;
             if (NV % 4 != 0 && q >= NV) break;
-            const int c = q >> 1;
+            const int u = v_part(q), c = v_dims(q);
 #pragma unroll
             for (int t = 0; t < 4; t += 2) {   // columns t and t + 1
                 if (REM && c >= NC && t > 0) break;
@@ -870,9 +901,9 @@ struct TilePart {
                 const uint4 uh = __builtin_bit_cast(uint4, hi), ul = __builtin_bit_cast(uint4, lo);
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    const int tt = 4 * c + t + w;
-                    lv[((2 * tt + 0) * 64 + lane) * 2 + (q & 1)] = w ? make_uint2(uh.z, uh.w) : make_uint2(uh.x, uh.y);
-                    lv[((2 * tt + 1) * 64 + lane) * 2 + (q & 1)] = w ? make_uint2(ul.z, ul.w) : make_uint2(ul.x, ul.y);
+                    const int tt = (u >> 1) * DT + 4 * c + t + w;
+                    lv[((2 * tt + 0) * 64 + lane) * 2 + (u & 1)] = w ? make_uint2(uh.z, uh.w) : make_uint2(uh.x, uh.y);
+                    lv[((2 * tt + 1) * 64 + lane) * 2 + (u & 1)] = w ? make_uint2(ul.z, ul.w) : make_uint2(ul.x, ul.y);
                 }
             }
         }
@@ -885,11 +916,11 @@ struct TilePart {
 template <int D, int MT, bool Q8, bool OWN>
 __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int item, int h, int split) {
     using T = TilePart<D, Q8>;
-    constexpr int KS = D / 32, DT = D / 16, NK = T::NK, kTileU4 = T::kBytes / 16;
+    constexpr int KS = D / 32, DT = D / 16, NK = T::NK, NU = T::NU, TR = 16 * NU, kTileU4 = T::kBytes / 16;
     constexpr bool TWO = wide_tiles(D) == 2;
     __shared__ int s_range[4][kAttnWaves];
-    __shared__ float s_max[2][2][kAttnWaves];
-    __shared__ unsigned s_bad[2][kAttnWaves];
+    __shared__ unsigned s_max[2][kAttnWaves], s_gone[2][kAttnWaves];
+    __shared__ unsigned long long s_bad[2][kAttnWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
     const ItemRows x = item_rows<OWN>(a, item, 64 * MT, lane);
     if (x.r0 >= x.r1) return;
@@ -937,87 +968,123 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
     else hi = min(a.prefix, hi);
     int t_lo, t_hi;
     split_tiles<OWN>(a, lo, hi, split, t_lo, t_hi);
+    // The split's rows [lo, hi), taken TR at a time from row0 on.
+    const int row0 = t_lo * kTile, tiles = (t_hi - t_lo + TR / kTile - 1) / (TR / kTile);
+    lo = max(lo, row0);
+    hi = min(hi, t_hi * kTile);
 
     int ev = -1000;
     const int rmask = (1 << a.pool.shift) - 1;
-    auto entry = [&](int tile, int u) { return x.blk[min((tile * kTile + 16 * u) >> a.pool.shift, a.width - 1)]; };
+    // Entries of the block table for the 16-row parts, each of which lies in one page; one outside the
+    // pool holds no rows (page 0 is read instead and masked).
+    auto entry = [&](int tile, int u) { return x.blk[min((row0 + tile * TR + 16 * u) >> a.pool.shift, a.width - 1)]; };
     auto in_pool = [&](int e) { return paged_page_ok(e, a.pool.n_pages); };
-    // The loaded tile t (its pages c0, c1), the next one's table entries n0, n1.
+    // The loaded tile t, its pages' entries c, and the next one's e: of the wave's parts.
     T t;
-    int n0 = 0, n1 = 0, c0 = 0, c1 = 0;
-    auto load = [&](int tile) {
-        c0 = __builtin_amdgcn_readfirstlane(n0);
-        c1 = __builtin_amdgcn_readfirstlane(n1);
-        n0 = entry(tile + 1, 0);
-        n1 = entry(tile + 1, 1);
-        t.load(a.pool, in_pool(c0) ? c0 : 0, in_pool(c1) ? c1 : 0, h, tile * kTile & rmask, (tile * kTile + 16) & rmask, wave, n, g);
+    int ek[T::KP] = {}, ev_[T::VP] = {}, ck[T::KP] = {}, cv[T::VP] = {};
+    auto entries = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < T::KP; ++i) ek[i] = entry(tile, T::k_part(wave + 4 * i));
+#pragma unroll
+        for (int i = 0; i < T::VP; ++i) ev_[i] = entry(tile, T::v_part(wave + 4 * i));
     };
+    auto load = [&](int tile) {
+        int pk_[T::KP], pv_[T::VP];
+#pragma unroll
+        for (int i = 0; i < T::KP; ++i) {
+            ck[i] = __builtin_amdgcn_readfirstlane(ek[i]);
+            pk_[i] = in_pool(ck[i]) ? ck[i] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < T::VP; ++i) {
+            cv[i] = __builtin_amdgcn_readfirstlane(ev_[i]);
+            pv_[i] = in_pool(cv[i]) ? cv[i] : 0;
+        }
+        entries(tile + 1);
+        t.load(a.pool, pk_, pv_, [&](int u) { return (row0 + tile * TR + 16 * u) & rmask; }, h, wave, n, g);
+    };
+    // Parts of the loaded tile that no page of the pool holds, of those that the wave loads.
+    auto parts_gone = [&]() {
+        unsigned y = 0;
+#pragma unroll
+        for (int i = 0; i < T::KP; ++i)
+            if (T::NK % 4 == 0 || wave + 4 * i < T::NK) y |= (unsigned)!in_pool(ck[i]) << T::k_part(wave + 4 * i);
+#pragma unroll
+        for (int i = 0; i < T::VP; ++i)
+            if (T::NV % 4 == 0 || wave + 4 * i < T::NV) y |= (unsigned)!in_pool(cv[i]) << T::v_part(wave + 4 * i);
+        return y;
+    };
+    auto held = [&](int k0, unsigned gone, int row) { return !(gone >> (row >> 4) & 1) && k0 + row >= lo && k0 + row < hi; };
     // The loaded tile's largest values, for the exponents; and where some query does not attend all of
     // it, or a value is infinite, what is not to be multiplied is taken out.
     auto inspect = [&](int tile) {
-        const int k0 = tile * kTile, slot = (tile - t_lo) & 1;
-        const bool there0 = in_pool(c0), there1 = in_pool(c1);
-        unsigned bad = 0;
-        float mk = wave_max(t.max_k(wave)), mv = wave_max(t.max_v(wave));
-        const bool every = k0 >= max(lo, lo_every) && k0 + kTile <= min(hi, hi_every) && there0 && there1;
-        if (!every || !finite_bits(__float_as_uint(mk)) || !finite_bits(__float_as_uint(mv))) {
-            auto held = [&](int row) { return (row < 16 ? there0 : there1) && k0 + row >= lo && k0 + row < hi; };
-            bad = t.clean(held, wave, n, g);
-            bad = __ballot(bad) != 0 ? wave_or(bad) : 0u;
-            mk = wave_max(t.max_k(wave));
-            mv = wave_max(t.max_v(wave));
+        const int k0 = row0 + tile * TR;
+        const unsigned gone = parts_gone();
+        unsigned long long bad = 0;
+        unsigned mx = t.largest(wave);
+        const bool every = k0 >= max(lo, lo_every) && k0 + TR <= min(hi, hi_every) && gone == 0;
+        if (!every || (mx & 0x7F80u) == 0x7F80u || mx >= 0x7F800000u) {
+            bad = t.clean([&](int row) { return held(k0, gone, row); }, wave, n, g);
+            bad = __ballot(bad != 0) != 0
+                      ? (unsigned long long)wave_or((unsigned)(bad >> 32)) << 32 | wave_or((unsigned)bad) : 0ull;
+            mx = t.largest(wave);
         }
         if (lane == 0) {
-            s_max[slot][0][wave] = mk;
-            s_max[slot][1][wave] = mv;
-            s_bad[slot][wave] = bad;
+            s_max[tile & 1][wave] = mx;
+            s_bad[tile & 1][wave] = bad;
+            s_gone[tile & 1][wave] = gone;
         }
     };
     // The inspected tile to LDS, and what its multiplication has to know.
     struct Stored {
         int ek;
-        float fe;             // factor of the outputs that V's exponent brings
-        unsigned poison;      // rows (bit = row of the tile) that hold a value that is not finite
-        bool there0, there1;
+        float fe;                    // factor of the outputs that V's exponent brings
+        unsigned long long poison;   // rows (bit = row of the tile) that hold a value that is not finite
+        unsigned gone;               // 16-row parts that no page of the pool holds
     };
     auto store = [&](int tile) {
-        const int slot = (tile - t_lo) & 1;
-        const float(&y)[2][kAttnWaves] = s_max[slot];
-        const float ak = fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3]));
-        const float av = fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3]));
+        const unsigned(&y)[kAttnWaves] = s_max[tile & 1];
+        const unsigned mx = __builtin_amdgcn_readfirstlane(max_halves(max_halves(y[0], y[1]), max_halves(y[2], y[3])));
+        const unsigned long long(&z)[kAttnWaves] = s_bad[tile & 1];
+        const unsigned long long bad = z[0] | z[1] | z[2] | z[3];
         Stored r;
-        r.poison = __builtin_amdgcn_readfirstlane(s_bad[slot][0] | s_bad[slot][1] | s_bad[slot][2] | s_bad[slot][3]);
-        r.ek = __builtin_amdgcn_readfirstlane(fit_exp(ak));
-        r.fe = raise_exp(ev, __builtin_amdgcn_readfirstlane(fit_exp(av)));
-        r.there0 = in_pool(c0);
-        r.there1 = in_pool(c1);
-        t.store(lds + (TWO ? slot * kTileU4 : 0), pk::pow2i(-r.ek), pk::pow2i(-ev), wave, lane);
+        r.poison = (unsigned long long)__builtin_amdgcn_readfirstlane((unsigned)(bad >> 32)) << 32 |
+                   (unsigned)__builtin_amdgcn_readfirstlane((unsigned)bad);
+        // (Q8: the largest scales, whose quants reach 128)
+        r.ek = fit_exp(__uint_as_float(mx << 16)) + (Q8 ? 7 : 0);
+        r.fe = raise_exp(ev, fit_exp(__uint_as_float(mx & 0xFFFF0000u)) + (Q8 ? 7 : 0));
+        const unsigned(&w)[kAttnWaves] = s_gone[tile & 1];
+        r.gone = __builtin_amdgcn_readfirstlane(w[0] | w[1] | w[2] | w[3]);
+        t.store(lds + (TWO ? (tile & 1) * kTileU4 : 0), pk::pow2i(-r.ek), pk::pow2i(-ev), wave, lane);
         return r;
     };
     auto multiply = [&](int tile, const Stored& now) {
         if (rw >= x.r1) return;   // no rows of its own: only the loads are its work
-        const int k0 = tile * kTile;
-        const f16x8* op = reinterpret_cast<const f16x8*>(lds + (TWO ? ((tile - t_lo) & 1) * kTileU4 : 0));
-        floatx4 st[MT][2];
+        const int k0 = row0 + tile * TR;
+        const f16x8* op = reinterpret_cast<const f16x8*>(lds + (TWO ? (tile & 1) * kTileU4 : 0));
+        floatx4 st[MT][NU];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) st[mt][0] = st[mt][1] = floatx4{0, 0, 0, 0};
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) st[mt][u] = floatx4{0, 0, 0, 0};
 #pragma unroll
         for (int q = 0; q < NK; ++q) {
             const f16x8 kh = op[2 * q * 64 + lane], kl = op[(2 * q + 1) * 64 + lane];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                floatx4& c = st[mt][q / KS];
-                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[mt][q % KS], c, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[mt][q % KS], c, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[mt][q % KS], c, 0, 0, 0);
+                floatx4& y = st[mt][q / KS];
+                y = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[mt][q % KS], y, 0, 0, 0);
+                y = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[mt][q % KS], y, 0, 0, 0);
+                y = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[mt][q % KS], y, 0, 0, 0);
             }
         }
-        auto held = [&](int row) { return (row < 16 ? now.there0 : now.there1) && k0 + row >= lo && k0 + row < hi; };
-        auto attended = [&](int mt, int row) { return held(row) && k0 + row >= first[mt] && k0 + row <= pos[mt]; };
-        const bool plain = k0 >= max(lo, lo_all) && k0 + kTile <= min(hi, hi_all) && now.there0 && now.there1;
-        f16x8 ph[MT], pl[MT];
+        auto attended = [&](int mt, int row) {
+            return held(k0, now.gone, row) && k0 + row >= first[mt] && k0 + row <= pos[mt];
+        };
+        const bool plain = k0 >= max(lo, lo_all) && k0 + TR <= min(hi, hi_all) && now.gone == 0 && now.poison == 0;
+        f16x8 ph[MT][NU / 2], pl[MT][NU / 2];
         const bool rescale =
-            tile_softmax<MT>(a, st, pk::pow2i(now.ek), fq, m, l, alpha, ph, pl, !plain || now.poison, now.poison, g, attended);
+            tile_softmax<MT, NU>(a, st, pk::pow2i(now.ek), fq, m, l, alpha, ph, pl, !plain, now.poison, g, attended);
         if (rescale || now.fe != 1.0f) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -1027,49 +1094,51 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
             }
         }
 #pragma unroll
-        for (int tt = 0; tt < DT; ++tt) {
-            const f16x8 vh = op[(NK + tt) * 2 * 64 + lane], vl = op[((NK + tt) * 2 + 1) * 64 + lane];
+        for (int w = 0; w < NU / 2; ++w)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[mt], o[mt][tt], 0, 0, 0);
-                o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[mt], o[mt][tt], 0, 0, 0);
-                o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[mt], o[mt][tt], 0, 0, 0);
+            for (int tt = 0; tt < DT; ++tt) {
+                const int q = NK + w * DT + tt;
+                const f16x8 vh = op[q * 2 * 64 + lane], vl = op[(q * 2 + 1) * 64 + lane];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[mt][w], o[mt][tt], 0, 0, 0);
+                    o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[mt][w], o[mt][tt], 0, 0, 0);
+                    o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[mt][w], o[mt][tt], 0, 0, 0);
+                }
             }
-        }
     };
-    if (t_lo < t_hi) {
-        n0 = entry(t_lo, 0);
-        n1 = entry(t_lo, 1);
-        load(t_lo);
-        inspect(t_lo);
+    if (tiles > 0) {
+        entries(0);
+        load(0);
+        inspect(0);
     }
     __syncthreads();
     if constexpr (TWO) {
         Stored now{};
-        if (t_lo < t_hi) {
-            now = store(t_lo);
-            if (t_lo + 1 < t_hi) {
-                load(t_lo + 1);
-                inspect(t_lo + 1);
+        if (tiles > 0) {
+            now = store(0);
+            if (tiles > 1) {
+                load(1);
+                inspect(1);
             }
         }
         __syncthreads();
-        for (int tile = t_lo; tile < t_hi; ++tile) {
+        for (int tile = 0; tile < tiles; ++tile) {
             Stored next = now;
-            if (tile + 1 < t_hi) next = store(tile + 1);   // into the tile that was multiplied before the barrier
-            if (tile + 2 < t_hi) load(tile + 2);
+            if (tile + 1 < tiles) next = store(tile + 1);   // over the tile that was multiplied before the barrier
+            if (tile + 2 < tiles) load(tile + 2);
             multiply(tile, now);
-            if (tile + 2 < t_hi) inspect(tile + 2);
+            if (tile + 2 < tiles) inspect(tile + 2);
             now = next;
             __syncthreads();
         }
     } else {
-        for (int tile = t_lo; tile < t_hi; ++tile) {
+        for (int tile = 0; tile < tiles; ++tile) {
             const Stored now = store(tile);
-            if (tile + 1 < t_hi) load(tile + 1);
+            if (tile + 1 < tiles) load(tile + 1);
             __syncthreads();
             multiply(tile, now);
-            if (tile + 1 < t_hi) inspect(tile + 1);
+            if (tile + 1 < tiles) inspect(tile + 1);
             __syncthreads();
         }
     }
@@ -1089,6 +1158,12 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
 // one another and share that part's L2.
 __device__ __forceinline__ int by_part(int id, int count) { return (id & 7) * (count >> 3) + (id >> 3); }
 
+// Dynamic LDS: the tiles of attn_wide, or the waves' states that attn_narrow joins.
+template <int D>
+constexpr size_t attn_lds(int wide) {
+    return wide ? (size_t)wide_tiles(D) * TilePart<D, false>::kBytes : 2 * (size_t)(D / 4 + 2) * 64 * 4;
+}
+
 // WIDE 0: items of 16 query rows; else of 64*WIDE.
 template <int D, int WIDE, bool Q8, bool OWN>
 __device__ __forceinline__ void attn_item(const AttnArgs& a, uint4* lds, int item, int h, int split) {
@@ -1100,7 +1175,7 @@ __device__ __forceinline__ void attn_item(const AttnArgs& a, uint4* lds, int ite
 // head), the others the own rows' (item of item_sequence, split, KV head): one launch, so the one fills
 // what the other leaves of the chip.
 template <int D, int WP, int WO, bool Q8>
-__global__ __launch_bounds__(kAttnThreads, 2) void paged_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads, D > 128 ? 1 : 2) void paged_attn_kernel(AttnArgs a) {
     extern __shared__ uint4 s_dyn4[];
     int id = blockIdx.x;
     if (id < a.prefix_wgs) {

@@ -129,10 +129,11 @@ LLMP_HD inline int paged_item_base(int start, int group, int rows, int b) {
 }
 
 // ---- launch plan -------------------------------------------------------------------------------
-// Query rows of a work item: 16 (wide 0), or 64 or 128 (wide 1, 2; at head_dim 256 the outputs of 128
-// do not fit the registers).
+// Query rows of a work item: 16 (wide 0), or 64 or 128 (wide 1, 2).  At head_dim 256 neither the rows
+// that a wave of the 16 takes by itself nor the outputs of 128 fit the registers.
 LLMP_HD constexpr int paged_item_rows(int wide) { return wide ? 64 * wide : 16; }
 constexpr int paged_wide_max(int head_dim) { return head_dim > 128 ? 1 : 2; }
+constexpr bool paged_narrow(int head_dim) { return head_dim <= 128; }
 
 struct PagedPlan {
     int prefix_wide, prefix_splits, prefix_tiles;   // item size, splits, 32-row tiles of a split
@@ -144,11 +145,12 @@ struct PagedPlan {
 inline PagedPlan paged_plan(int n_seqs, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int prefix, int max_len,
                             int n_cu) {
     const long long cu = n_cu > 0 ? n_cu : 256, group = n_heads / n_kv_heads, rows = (long long)n_tokens * group;
-    auto wide_of = [&](long long r) { return r <= 16 ? 0 : r <= 64 ? 1 : paged_wide_max(head_dim); };
+    auto wide_of = [&](long long r) { return r <= 16 && paged_narrow(head_dim) ? 0 : r <= 64 ? 1 : paged_wide_max(head_dim); };
     auto items_of = [&](long long r, int wide) { return (r + paged_item_rows(wide) - 1) / paged_item_rows(wide); };
-    // About two workgroups a CU, with at least 8 tiles of 32 rows a split.
-    auto splits_of = [&](long long tiles, long long items) {
-        return (int)std::max<long long>(1, std::min((2 * cu + items - 1) / items, (tiles + 7) / 8));
+    // About two workgroups a CU for the prefix and three for the own rows, whose lengths differ, with at
+    // least 4 tiles of 32 rows a split.
+    auto splits_of = [&](long long tiles, long long items, int per_cu) {
+        return (int)std::max<long long>(1, std::min((per_cu * cu + items - 1) / items, (tiles + 3) / 4));
     };
     PagedPlan p{};
     const long long each = (rows + n_seqs - 1) / n_seqs;
@@ -156,11 +158,11 @@ inline PagedPlan paged_plan(int n_seqs, int n_tokens, int n_heads, int n_kv_head
     p.own_wide = wide_of(each);
     if (prefix > 0) {
         const long long tiles = (prefix + 31) / 32;
-        const int s = splits_of(tiles, items_of(rows, p.prefix_wide) * n_kv_heads);
+        const int s = splits_of(tiles, items_of(rows, p.prefix_wide) * n_kv_heads, 2);
         p.prefix_tiles = (int)((tiles + s - 1) / s);
         p.prefix_splits = (int)((tiles + p.prefix_tiles - 1) / p.prefix_tiles);
     }
-    p.own_splits = splits_of((std::max(max_len - prefix, 1) + 31) / 32, n_seqs * items_of(each, p.own_wide) * n_kv_heads);
+    p.own_splits = splits_of((std::max(max_len - prefix, 1) + 31) / 32, n_seqs * items_of(each, p.own_wide) * n_kv_heads, 3);
     return p;
 }
 
