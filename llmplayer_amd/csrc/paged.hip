@@ -14,9 +14,21 @@ hipError_t allow_lds(K kernel, size_t bytes) {
     return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
+template <int D, bool F32, bool Q8>
+hipError_t launch_append_registers(const pg::AppendArgs& a, int all, hipStream_t st) {
+    constexpr int per = pg::kAppendThreads / (D / 8);
+    hipLaunchKernelGGL((pg::paged_append_kernel<D, F32, Q8>), dim3(a.n_tokens, (all + per - 1) / per), dim3(pg::kAppendThreads),
+                       0, st, a);
+    return hipGetLastError();
+}
+
 template <int D>
 hipError_t launch_append_d(const pg::AppendArgs& a, hipStream_t st) {
     const int all = a.k != nullptr ? a.n_heads + 2 * a.pool.n_kv_heads : a.n_heads;
+    if (pg::append_in_registers(a, D)) {
+        if (a.in_f32) return a.q8 ? launch_append_registers<D, true, true>(a, all, st) : launch_append_registers<D, true, false>(a, all, st);
+        return a.q8 ? launch_append_registers<D, false, true>(a, all, st) : launch_append_registers<D, false, false>(a, all, st);
+    }
     hipLaunchKernelGGL((pg::paged_append_lds_kernel<D>), dim3(a.n_tokens, (all + pg::kAppendHeads - 1) / pg::kAppendHeads),
                        dim3(pg::kAppendThreads), 0, st, a);
     return hipGetLastError();

@@ -169,13 +169,114 @@ __device__ __forceinline__ floatx4 load4_in(const void* p, long long i, int f32)
 // unit in the last place of the division, which moves a quant only at a border between two).  Truncated
 // ones take a contiguous cache's division: there the last place decides the quant of the largest value.
 constexpr float kInv127 = 1.0f / 127.0f;
+__device__ __forceinline__ float q8_scale(float mx, bool trunc) { return trunc ? mx / 127.0f : mx * kInv127; }
 __device__ __forceinline__ float block_scale(const float* x, bool trunc) {
     float mx = 0.0f;
     for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fabsf(x[i]));
-    return trunc ? mx / 127.0f : mx * kInv127;
+    return q8_scale(mx, trunc);
 }
 
-// One workgroup = (token, group of kAppendHeads heads): the heads [h0, h0 + kAppendHeads) of the token's
+// Whether a call takes the register kernel: no norm (whose sums run over a head in a fixed order), rows
+// that load in fours, and pairs and quantised blocks that lie in the lanes as that kernel has them.
+inline bool append_in_registers(const AppendArgs& a, int D) {
+    const uintptr_t row = a.in_f32 ? 15 : 7;
+    const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+    if (a.qnw != nullptr || a.knw != nullptr || a.v_norm) return false;
+    if ((at(a.q) | at(a.k) | at(a.v)) & row || at(a.out) & 15) return false;
+    if ((a.q_stride | a.k_stride | a.v_stride | a.out_stride | (a.cos_t ? a.half_rope : 0)) & 3) return false;
+    const bool halves = a.cos_t != nullptr && a.rope_type != 0;
+    return !a.q8 || !halves || a.half_rope <= 16 || (a.half_rope % 32 == 0 && D % 64 == 0);
+}
+
+// Without a norm.  A thread holds 8 values of a head, two fours that rotate within themselves (adjacent
+// pairs) or with each other (halves: [i, i + 4) and [half + i, half + i + 4)), from their load to their store.
+// A quantised block of 32 lies in 4 lanes (both fours), or in 8 lanes (the fours of two blocks): its maximum
+// takes two or three lane exchanges.  Bound by HBM: every value is read once and written once (4099 tokens
+// of 32 + 8 + 8 heads of 128, bf16 to fp32: 26 us, 5.8 TB/s; through LDS 55 us.  1500 tokens of
+// 32 + 8 + 8 heads of 64, fp32 to Q8_0: 8 us, through LDS 17 us).
+template <int D, bool F32, bool Q8>
+__global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a) {
+    constexpr int TPH = D / 8, HPW = kAppendThreads / TPH;   // threads of a head, heads of a workgroup
+    const int t = blockIdx.x, j = threadIdx.x % TPH;
+    const int hh = blockIdx.y * HPW + threadIdx.x / TPH;
+    const int Hq = a.n_heads, Hkv = a.pool.n_kv_heads;
+    if (threadIdx.x >= TPH * HPW || hh >= (a.k != nullptr ? Hq + 2 * Hkv : Hq)) return;
+    const bool is_q = hh < Hq, is_k = !is_q && hh < Hq + Hkv;
+    const int h = is_q ? hh : is_k ? hh - Hq : hh - Hq - Hkv;
+    const bool rope = a.cos_t != nullptr && (is_q || is_k), halves = rope && a.rope_type != 0;
+    const int half = rope ? a.half_rope : 0;
+    const bool rot = 4 * j < half, apart = halves && rot;
+    const int ea = apart ? 4 * j : 8 * j, eb = apart ? half + 4 * j : ea + 4;
+    const void* in = is_q ? a.q : is_k ? a.k : a.v;
+    const long long row = (is_q ? a.q_stride : is_k ? a.k_stride : a.v_stride) * t + h * D;
+    floatx4 xa = load4_in(in, row + ea, F32), xb = load4_in(in, row + eb, F32);
+    const int pos = a.positions[t];
+    if ((unsigned)pos >= (unsigned)a.max_seq) return;
+    if (rot) {
+        const floatx4 c = *reinterpret_cast<const floatx4*>(a.cos_t + (long long)pos * half + 4 * j);
+        const floatx4 s = *reinterpret_cast<const floatx4*>(a.sin_t + (long long)pos * half + 4 * j);
+        float x0[4], x1[4], y0[4], y1[4];   // the pairs
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const floatx4& x = i < 2 ? xa : xb;
+            x0[i] = halves ? xa[i] : x[2 * (i & 1)];
+            x1[i] = halves ? xb[i] : x[2 * (i & 1) + 1];
+            const float t0 = x0[i] * c[i], t1 = x1[i] * s[i], t2 = x0[i] * s[i], t3 = x1[i] * c[i];
+            y0[i] = t0 - t1;
+            y1[i] = t2 + t3;
+        }
+        xa = halves ? floatx4{y0[0], y0[1], y0[2], y0[3]} : floatx4{y0[0], y1[0], y0[1], y1[1]};
+        xb = halves ? floatx4{y1[0], y1[1], y1[2], y1[3]} : floatx4{y0[2], y1[2], y0[3], y1[3]};
+    }
+    if (is_q) {
+        float* o = a.out + a.out_stride * t + h * D;
+        *reinterpret_cast<floatx4*>(o + ea) = xa;
+        *reinterpret_cast<floatx4*>(o + eb) = xb;
+        return;
+    }
+    const int slot = a.slots[t];
+    if (!paged_slot_ok(slot, a.pool.shift, a.pool.n_pages)) return;
+    const long long to = ((((long long)(slot >> a.pool.shift) * Hkv + h) << a.pool.shift) + (slot & ((1 << a.pool.shift) - 1)));
+    void* plane = is_k ? a.pool.k : a.pool.v;
+    if constexpr (!Q8) {
+        float* o = static_cast<float*>(plane) + to * D;
+        *reinterpret_cast<floatx4*>(o + ea) = xa;
+        *reinterpret_cast<floatx4*>(o + eb) = xb;
+    } else {
+        auto largest = [](const floatx4& x) {
+            return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+        };
+        auto over_four = [](float x) {
+            x = fmaxf(x, dk::dpp<dk::kDppQuadXor1>(x));
+            return fmaxf(x, dk::dpp<dk::kDppQuadXor2>(x));
+        };
+        const bool eight = apart && half % 32 == 0;
+        float ma = largest(xa), mb = largest(xb);
+        if (!eight) ma = mb = fmaxf(ma, mb);
+        ma = over_four(ma);
+        mb = over_four(mb);
+        if (eight) {
+            ma = fmaxf(ma, dk::dpp<dk::kDppRowHalfMirror>(ma));
+            mb = fmaxf(mb, dk::dpp<dk::kDppRowHalfMirror>(mb));
+        }
+        const float sa = q8_scale(ma, a.q8_trunc != 0), sb = q8_scale(mb, a.q8_trunc != 0);
+        float* so = (is_k ? a.pool.ks : a.pool.vs) + to * (D / 32);
+        if ((ea & 31) == 0) so[ea / 32] = sa;
+        if (eight && (eb & 31) == 0) so[eb / 32] = sb;
+        const float ia = dk::q8_inv_scale(sa), ib = dk::q8_inv_scale(sb);
+        unsigned wa = 0, wb = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            wa |= (unsigned)(dk::q8_code(xa[i], ia, a.q8_trunc != 0) & 0xFF) << (8 * i);
+            wb |= (unsigned)(dk::q8_code(xb[i], ib, a.q8_trunc != 0) & 0xFF) << (8 * i);
+        }
+        signed char* o = static_cast<signed char*>(plane) + to * D;
+        *reinterpret_cast<unsigned*>(o + ea) = wa;
+        *reinterpret_cast<unsigned*>(o + eb) = wb;
+    }
+}
+
+// The others (norms, odd strides).  One workgroup = (token, group of kAppendHeads heads): the heads [h0, h0 + kAppendHeads) of the token's
 // query, key and value heads in that order, staged in LDS and prepared with the decode path's
 // functions, so the rows are bit-identical to a decode append's (before they are quantised).
 constexpr int kAppendHeads = 8;

@@ -63,6 +63,13 @@ CASES = [
     (16, 8, 128, 16, 11, 2, 64, False, 0, 1, False, False),
     (16, 8, 64, 16, 11, 2, 16, False, 0, 2, True, False),
     (8, 2, 256, 64, 4, 0, 64, False, 2, 0, False, False),
+    (8, 2, 256, 64, 7, 2, 256, False, 0, 1, False, False),
+    (16, 8, 128, 16, 13, 2, 128, False, 0, 2, False, True),
+    (16, 8, 128, 16, 13, 2, 48, False, 0, 1, False, False),
+    (32, 8, 64, 32, 70, 2, 32, False, 0, 1, True, True),
+    (24, 8, 96, 16, 7, 2, 96, False, 0, 1, False, False),
+    (24, 8, 96, 16, 7, 2, 64, False, 0, 1, True, False),
+    (24, 8, 96, 16, 7, 0, 96, False, 0, 2, False, False),
 ]
 
 
@@ -148,6 +155,41 @@ def test_append(hq, hkv, D, page, T, rope_type, rope_dim, norm, norm_mode, cache
         finally:
             kv.destroy()
             ref.destroy()
+
+
+@pytest.mark.parametrize("D,rope_type,rope_dim,cache,bf16", [
+    (64, 0, 64, 0, False), (64, 2, 64, 1, True), (128, 2, 128, 1, False), (128, 0, 64, 2, True), (96, 0, 96, 1, False),
+    (256, 2, 24, 0, True), (128, 0, 0, 1, False)])
+def test_every_alignment_stores_the_same(D, rope_type, rope_dim, cache, bf16):
+    """Rows that load in fours and rows at odd strides and offsets: the same bytes out of both."""
+    rng = np.random.default_rng(D + rope_dim)
+    hq, hkv, page, n_pages, T = 6, 3, 16, 3, 33
+    tables = hfp.rope_table(rope_dim, MAX_SEQ, 1e5) if rope_dim else None
+    rows = rng.standard_normal((T, (hq + 2 * hkv) * D)).astype(F32)
+    raw = hfp.to_bf16(rows).reshape(rows.shape) if bf16 else rows
+    positions, slots = rng.permutation(MAX_SEQ)[:T].astype(I), rng.permutation(n_pages * page)[:T].astype(I)
+    cut = np.cumsum([0, hq * D, hkv * D, hkv * D])
+    seen = []
+    for pad, first in ((0, 0), (8, 0), (1, 0), (3, 1), (4, 2)):
+        with pc.Device() as d:
+            kv = PagedKv(1, n_pages, page, MAX_SEQ, hkv, D, cache)
+            try:
+                config(kv.handle, hq, hkv, D, rope_type, rope_dim, None, None, 0, tables)
+                kv.write(0, {w: np.zeros(s, t) for w, (s, t) in kv._shapes().items()})
+                held = np.zeros((T, raw.shape[1] + pad), raw.dtype)
+                held[:, :raw.shape[1]] = raw
+                flat = np.concatenate([np.zeros(first, raw.dtype), held.reshape(-1)])
+                base, stride, size = d.up(flat) + first * raw.itemsize, held.shape[1], raw.itemsize
+                out = d.up(np.zeros((T, hq * D + pad), F32))
+                _lib.call("llmp_paged_append", kv.handle, 0, T, d.up(positions), d.up(slots), 1 if bf16 else 0,
+                          base, stride, base + int(cut[1]) * size, stride, base + int(cut[2]) * size, stride, out, hq * D + pad, 0)
+                got = kv.read(0)
+                got["q"] = d.down(out, F32, (T, hq * D + pad))[:, :hq * D]
+                seen.append({w: np.ascontiguousarray(x).view(np.uint8) for w, x in got.items()})
+            finally:
+                kv.destroy()
+    for other in seen[1:]:
+        assert all(np.array_equal(other[w], seen[0][w]) for w in seen[0])
 
 
 @pytest.mark.parametrize("norm", [False, True])
