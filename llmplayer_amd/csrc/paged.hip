@@ -17,8 +17,9 @@ hipError_t allow_lds(K kernel, size_t bytes) {
 template <int D, bool F32, bool Q8>
 hipError_t launch_append_registers(const pg::AppendArgs& a, int all, hipStream_t st) {
     constexpr int per = pg::kAppendThreads / (D / 8);
-    hipLaunchKernelGGL((pg::paged_append_kernel<D, F32, Q8>), dim3(a.n_tokens, (all + per - 1) / per), dim3(pg::kAppendThreads),
-                       0, st, a);
+    const dim3 grid(a.n_tokens, (all + per - 1) / per), block(pg::kAppendThreads);
+    if (a.qnw != nullptr) hipLaunchKernelGGL((pg::paged_append_kernel<D, F32, Q8, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((pg::paged_append_kernel<D, F32, Q8, false>), grid, block, 0, st, a);
     return hipGetLastError();
 }
 

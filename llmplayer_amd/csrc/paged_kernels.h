@@ -176,42 +176,90 @@ __device__ __forceinline__ float block_scale(const float* x, bool trunc) {
     return q8_scale(mx, trunc);
 }
 
-// Whether a call takes the register kernel: no norm (whose sums run over a head in a fixed order), rows
-// that load in fours, and pairs and quantised blocks that lie in the lanes as that kernel has them.
+// Whether a call takes the register kernel: no sum over a head that runs from its first value to its last
+// (LLMP_NORM_SEQUENTIAL's and the value norm's), rows that load in fours, and pairs and quantised blocks
+// that lie in the lanes as that kernel has them.
 inline bool append_in_registers(const AppendArgs& a, int D) {
     const uintptr_t row = a.in_f32 ? 15 : 7;
     const auto at = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
-    if (a.qnw != nullptr || a.knw != nullptr || a.v_norm) return false;
+    if ((a.qnw != nullptr && a.norm_seq) || a.v_norm) return false;
     if ((at(a.q) | at(a.k) | at(a.v)) & row || at(a.out) & 15) return false;
     if ((a.q_stride | a.k_stride | a.v_stride | a.out_stride | (a.cos_t ? a.half_rope : 0)) & 3) return false;
     const bool halves = a.cos_t != nullptr && a.rope_type != 0;
     return !a.q8 || !halves || a.half_rope <= 16 || (a.half_rope % 32 == 0 && D % 64 == 0);
 }
 
-// Without a norm.  A thread holds 8 values of a head, two fours that rotate within themselves (adjacent
+// A thread holds 8 values of a head, two fours that rotate within themselves (adjacent
 // pairs) or with each other (halves: [i, i + 4) and [half + i, half + i + 4)), from their load to their store.
 // A quantised block of 32 lies in 4 lanes (both fours), or in 8 lanes (the fours of two blocks): its maximum
 // takes two or three lane exchanges.  Bound by HBM: every value is read once and written once (4099 tokens
 // of 32 + 8 + 8 heads of 128, bf16 to fp32: 26 us, 5.8 TB/s; through LDS 55 us.  1500 tokens of
 // 32 + 8 + 8 heads of 64, fp32 to Q8_0: 8 us, through LDS 17 us).
-template <int D, bool F32, bool Q8>
+// NORM: a copy of the head in LDS gives the sum of its squares in the decode path's order, 8 chains of
+// every eighth value, added up one after the other (4099 tokens of 16 + 8 + 8 heads of 128, fp32: 53 us to
+// 28 us a call).
+template <int D, bool F32, bool Q8, bool NORM>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs a) {
     constexpr int TPH = D / 8, HPW = kAppendThreads / TPH;   // threads of a head, heads of a workgroup
     const int t = blockIdx.x, j = threadIdx.x % TPH;
     const int hh = blockIdx.y * HPW + threadIdx.x / TPH;
     const int Hq = a.n_heads, Hkv = a.pool.n_kv_heads;
-    if (threadIdx.x >= TPH * HPW || hh >= (a.k != nullptr ? Hq + 2 * Hkv : Hq)) return;
+    const bool live = threadIdx.x < TPH * HPW && hh < (a.k != nullptr ? Hq + 2 * Hkv : Hq);
+    if (!NORM && !live) return;
     const bool is_q = hh < Hq, is_k = !is_q && hh < Hq + Hkv;
     const int h = is_q ? hh : is_k ? hh - Hq : hh - Hq - Hkv;
     const bool rope = a.cos_t != nullptr && (is_q || is_k), halves = rope && a.rope_type != 0;
     const int half = rope ? a.half_rope : 0;
     const bool rot = 4 * j < half, apart = halves && rot;
     const int ea = apart ? 4 * j : 8 * j, eb = apart ? half + 4 * j : ea + 4;
-    const void* in = is_q ? a.q : is_k ? a.k : a.v;
-    const long long row = (is_q ? a.q_stride : is_k ? a.k_stride : a.v_stride) * t + h * D;
-    floatx4 xa = load4_in(in, row + ea, F32), xb = load4_in(in, row + eb, F32);
     const int pos = a.positions[t];
-    if ((unsigned)pos >= (unsigned)a.max_seq) return;
+    floatx4 xa{}, xb{};
+    if (live) {
+        const void* in = is_q ? a.q : is_k ? a.k : a.v;
+        const long long row = (is_q ? a.q_stride : is_k ? a.k_stride : a.v_stride) * t + h * D;
+        xa = load4_in(in, row + ea, F32);
+        xb = load4_in(in, row + eb, F32);
+    }
+    if ((unsigned)pos >= (unsigned)a.max_seq) return;   // (the workgroup's: it has one token)
+    if constexpr (NORM) {
+        constexpr int LD = D + 8;   // the rows of a wave's 8 heads start in banks 8 apart
+        __shared__ __align__(16) float s_x[HPW * LD];
+        __shared__ float s_r[HPW];
+        const int lh = threadIdx.x / TPH;
+        floatx4 wa{}, wb{};
+        if (live) {
+            const float* w = is_q ? a.qnw : a.knw;
+            wa = *reinterpret_cast<const floatx4*>(w + ea);
+            wb = *reinterpret_cast<const floatx4*>(w + eb);
+        }
+        if (lh < HPW) {
+            *reinterpret_cast<floatx4*>(s_x + lh * LD + ea) = xa;
+            *reinterpret_cast<floatx4*>(s_x + lh * LD + eb) = xb;
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < HPW * 8; c += kAppendThreads) {   // whole groups of 8 lanes
+            const float* x = s_x + (c >> 3) * LD + (c & 7);
+            float acc = 0.0f;
+#pragma unroll
+            for (int k = 0; k < D / 8; ++k) acc = __builtin_fmaf(x[8 * k], x[8 * k], acc);
+            float sum = __shfl(acc, 0, 8);
+#pragma unroll
+            for (int ln = 1; ln < 8; ++ln) sum = sum + __shfl(acc, ln, 8);
+            float v = sum / (float)D;
+            v = v + a.eps;
+            if ((c & 7) == 0) s_r[c >> 3] = 1.0f / (float)__builtin_sqrt((double)v);
+        }
+        __syncthreads();
+        if (!live) return;
+        if (is_q || is_k) {
+            const float r = s_r[lh];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                xa[i] = (xa[i] * r) * wa[i];
+                xb[i] = (xb[i] * r) * wb[i];
+            }
+        }
+    }
     if (rot) {
         const floatx4 c = *reinterpret_cast<const floatx4*>(a.cos_t + (long long)pos * half + 4 * j);
         const floatx4 s = *reinterpret_cast<const floatx4*>(a.sin_t + (long long)pos * half + 4 * j);
@@ -276,7 +324,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs
     }
 }
 
-// The others (norms, odd strides).  One workgroup = (token, group of kAppendHeads heads): the heads [h0, h0 + kAppendHeads) of the token's
+// The others (sequential norms, odd strides, blocks that do not lie in whole lanes).  One workgroup = (token, group of kAppendHeads heads): the heads [h0, h0 + kAppendHeads) of the token's
 // query, key and value heads in that order, staged in LDS and prepared with the decode path's
 // functions, so the rows are bit-identical to a decode append's (before they are quantised).
 constexpr int kAppendHeads = 8;

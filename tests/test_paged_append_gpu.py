@@ -157,10 +157,10 @@ def test_append(hq, hkv, D, page, T, rope_type, rope_dim, norm, norm_mode, cache
             ref.destroy()
 
 
-@pytest.mark.parametrize("D,rope_type,rope_dim,cache,bf16", [
-    (64, 0, 64, 0, False), (64, 2, 64, 1, True), (128, 2, 128, 1, False), (128, 0, 64, 2, True), (96, 0, 96, 1, False),
-    (256, 2, 24, 0, True), (128, 0, 0, 1, False)])
-def test_every_alignment_stores_the_same(D, rope_type, rope_dim, cache, bf16):
+@pytest.mark.parametrize("D,rope_type,rope_dim,cache,bf16,norm", [
+    (64, 0, 64, 0, False, False), (64, 2, 64, 1, True, True), (128, 2, 128, 1, False, False), (128, 0, 64, 2, True, True),
+    (96, 0, 96, 1, False, True), (256, 2, 24, 0, True, True), (128, 0, 0, 1, False, False)])
+def test_every_alignment_stores_the_same(D, rope_type, rope_dim, cache, bf16, norm):
     """Rows that load in fours and rows at odd strides and offsets: the same bytes out of both."""
     rng = np.random.default_rng(D + rope_dim)
     hq, hkv, page, n_pages, T = 6, 3, 16, 3, 33
@@ -169,12 +169,13 @@ def test_every_alignment_stores_the_same(D, rope_type, rope_dim, cache, bf16):
     raw = hfp.to_bf16(rows).reshape(rows.shape) if bf16 else rows
     positions, slots = rng.permutation(MAX_SEQ)[:T].astype(I), rng.permutation(n_pages * page)[:T].astype(I)
     cut = np.cumsum([0, hq * D, hkv * D, hkv * D])
+    qw, kw = ((rng.random(D) + 0.5).astype(F32) for _ in range(2)) if norm else (None, None)
     seen = []
     for pad, first in ((0, 0), (8, 0), (1, 0), (3, 1), (4, 2)):
         with pc.Device() as d:
             kv = PagedKv(1, n_pages, page, MAX_SEQ, hkv, D, cache)
             try:
-                config(kv.handle, hq, hkv, D, rope_type, rope_dim, None, None, 0, tables)
+                config(kv.handle, hq, hkv, D, rope_type, rope_dim, qw, kw, 0, tables)
                 kv.write(0, {w: np.zeros(s, t) for w, (s, t) in kv._shapes().items()})
                 held = np.zeros((T, raw.shape[1] + pad), raw.dtype)
                 held[:, :raw.shape[1]] = raw
