@@ -37,6 +37,7 @@ namespace pg {
 typedef pk::f16x8 f16x8;
 typedef pk::floatx4 floatx4;
 
+constexpr int kSchedAlu = 0x6;   // of the scheduler's barriers: VALU and scalar instructions may cross
 constexpr int kAttnThreads = 256, kAttnWaves = kAttnThreads / 64;
 constexpr int kTile = 32;            // pool rows a wave takes at a time
 constexpr float kPShift = 4.0f;      // 2^(s - m + 4): small probabilities keep their fp16 bits
@@ -347,9 +348,10 @@ __device__ __forceinline__ int fit_exp(float mx) {
 }
 
 __device__ __forceinline__ unsigned wave_or(unsigned x) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) x |= __shfl_xor(x, off);
-    return __builtin_amdgcn_readfirstlane(x);
+    return wave_reduce(x, [](unsigned a, unsigned b) { return a | b; });
+}
+__device__ __forceinline__ int wave_max_i(int x) {
+    return (int)wave_reduce((unsigned)x, [](unsigned a, unsigned b) { return (unsigned)max((int)a, (int)b); });
 }
 
 // The rows of a tile (bit = row) that the lanes' bits name: bk the K rows n and 16 + n, bv the V
@@ -358,17 +360,23 @@ __device__ __forceinline__ unsigned tile_rows(unsigned bk, unsigned bv, int n, i
     return wave_or((bk & 1u) << n | (bk >> 1) << (16 + n) | (bv & 15u) << (4 * g) | (bv >> 4) << (16 + 4 * g));
 }
 
-// The sequence of work item `item` of an own-rows launch (paged_item_base).
-__device__ __forceinline__ int item_sequence(const AttnArgs& a, int item, int BM, int lane) {
+// The sequence of work item `item` of an own-rows launch (paged_item_base), its start and its end: a search
+// by 64 lanes at once.
+__device__ __forceinline__ int item_sequence(const AttnArgs& a, int item, int BM, int lane, int& start, int& end) {
     int lo = 0, len = a.n_seqs;
-    while (len > 1) {
-        const int step = (len + 63) / 64, b = lo + lane * step;
-        const bool in = lane * step < len && paged_item_base(a.seq_start[b], a.group, BM, b) <= item;
+    for (;;) {
+        const int step = (len + 63) / 64, b = min(lo + lane * step, a.n_seqs - 1);
+        const int from = a.seq_start[b], to = a.seq_start[b + 1];
+        const bool in = lane * step < len && paged_item_base(from, a.group, BM, b) <= item;
         const int c = max((int)__popcll(__ballot(in)), 1) - 1;
         lo += c * step;
+        if (step == 1) {
+            start = __builtin_amdgcn_readlane(from, c);
+            end = __builtin_amdgcn_readlane(to, c);
+            return __builtin_amdgcn_readfirstlane(lo);
+        }
         len = min(step, len - c * step);
     }
-    return __builtin_amdgcn_readfirstlane(lo);
 }
 
 // The query rows of a work item: `rows` per item of one KV head, of all tokens (prefix) or of one
@@ -381,8 +389,10 @@ template <bool OWN>
 __device__ __forceinline__ ItemRows item_rows(const AttnArgs& a, int item, int rows, int lane) {
     ItemRows x{0, item * rows, 0, a.blocks};
     if constexpr (OWN) {
-        const int b = item_sequence(a, item, rows, lane);
-        const int st = min(max(a.seq_start[b], 0), a.n_tokens), en = min(max(a.seq_start[b + 1], st), a.n_tokens);
+        int st, en;
+        const int b = item_sequence(a, item, rows, lane, st, en);
+        st = min(max(st, 0), a.n_tokens);
+        en = min(max(en, st), a.n_tokens);
         x.tok0 = st;
         x.r0 = (item - paged_item_base(st, a.group, rows, b)) * rows;
         x.r1 = x.r0 < 0 ? x.r0 : min((en - st) * a.group, x.r0 + rows);
@@ -427,12 +437,6 @@ __device__ __forceinline__ void load_queries(const AttnArgs& a, const ItemRows& 
     pos = live ? p : -1;
     first = !live ? 0x7fffffff : a.window > 0 ? max(p + 1 - a.window, 0) : 0;
     fq = pk::pow2i(e);
-}
-
-__device__ __forceinline__ int wave_max_i(int x) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) x = max(x, __shfl_xor(x, off));
-    return __builtin_amdgcn_readfirstlane(x);
 }
 
 // The tiles [lo, hi) of one split of an item's rows [row_lo, row_hi).
@@ -1067,9 +1071,16 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int u = 0; u < NU; ++u) st[mt][u] = floatx4{0, 0, 0, 0};
+        // (Operand q + 1 is on its way out of LDS while q is multiplied.)
+        f16x8 xh = op[lane], xl = op[64 + lane];
 #pragma unroll
         for (int q = 0; q < NK; ++q) {
-            const f16x8 kh = op[2 * q * 64 + lane], kl = op[(2 * q + 1) * 64 + lane];
+            const f16x8 kh = xh, kl = xl;
+            if (q + 1 < NK) {
+                xh = op[(2 * q + 2) * 64 + lane];
+                xl = op[(2 * q + 3) * 64 + lane];
+            }
+            __builtin_amdgcn_sched_barrier(kSchedAlu);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 floatx4& y = st[mt][q / KS];
@@ -1093,19 +1104,24 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
                 for (int d = 0; d < DT; ++d) o[mt][d] = o[mt][d] * f;
             }
         }
+        xh = op[NK * 2 * 64 + lane];
+        xl = op[(NK * 2 + 1) * 64 + lane];
 #pragma unroll
-        for (int w = 0; w < NU / 2; ++w)
-#pragma unroll
-            for (int tt = 0; tt < DT; ++tt) {
-                const int q = NK + w * DT + tt;
-                const f16x8 vh = op[q * 2 * 64 + lane], vl = op[(q * 2 + 1) * 64 + lane];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[mt][w], o[mt][tt], 0, 0, 0);
-                    o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[mt][w], o[mt][tt], 0, 0, 0);
-                    o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[mt][w], o[mt][tt], 0, 0, 0);
-                }
+        for (int q = 0; q < NU / 2 * DT; ++q) {
+            const int w = q / DT, tt = q % DT;
+            const f16x8 vh = xh, vl = xl;
+            if (q + 1 < NU / 2 * DT) {
+                xh = op[(NK + q + 1) * 2 * 64 + lane];
+                xl = op[((NK + q + 1) * 2 + 1) * 64 + lane];
             }
+            __builtin_amdgcn_sched_barrier(kSchedAlu);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[mt][w], o[mt][tt], 0, 0, 0);
+                o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[mt][w], o[mt][tt], 0, 0, 0);
+                o[mt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[mt][w], o[mt][tt], 0, 0, 0);
+            }
+        }
     };
     if (tiles > 0) {
         entries(0);

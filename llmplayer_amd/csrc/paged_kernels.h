@@ -100,17 +100,13 @@ __global__ __launch_bounds__(kTablesThreads) void paged_tables_kernel(TablesArgs
         s_start[n] = tokens;
         s_need[n] = need;
         s_back[n] = back;
-        s_last = 1;
-        // All inputs of this workgroup are in LDS and registers (the barriers above): the last
-        // workgroup to come here may write over them.
-        if (gridDim.x > 1) {
-            __threadfence();
-            const int t = atomicAdd(a.ticket, 1);
-            s_last = t == (int)gridDim.x - 1;
-            if (s_last) *a.ticket = 0;
-        }
     }
     __syncthreads();
+    // All inputs of this workgroup are in LDS and registers: the last workgroup to come here may write over
+    // them.  (It writes over what the others have read and reads nothing of theirs: no fence; and the
+    // answer is not waited for before the end.)
+    int ticket = 0;
+    if (tid == 0 && gridDim.x > 1) ticket = atomicAdd(a.ticket, 1);
     // Entry e of the stack after the pushes, as the popping tokens see it.
     const int top = n_free + back;
     auto returned = [&](int r) {
@@ -143,6 +139,11 @@ __global__ __launch_bounds__(kTablesThreads) void paged_tables_kernel(TablesArgs
     }
     for (int r = g0; r < back; r += gn) a.free_pages[n_free + r] = returned(r);
     if (blockIdx.x == 0 && tid == 0) *a.status = status;
+    if (tid == 0) {
+        s_last = gridDim.x == 1 || ticket == (int)gridDim.x - 1;
+        if (s_last && gridDim.x > 1) *a.ticket = 0;
+    }
+    __syncthreads();
     if (s_last) {
         for (int i = tid; i < n; i += kTablesThreads) {
             const int l = s_len[i];

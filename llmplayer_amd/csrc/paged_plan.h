@@ -148,9 +148,14 @@ inline PagedPlan paged_plan(int n_seqs, int n_tokens, int n_heads, int n_kv_head
     auto wide_of = [&](long long r) { return r <= 16 && paged_narrow(head_dim) ? 0 : r <= 64 ? 1 : paged_wide_max(head_dim); };
     auto items_of = [&](long long r, int wide) { return (r + paged_item_rows(wide) - 1) / paged_item_rows(wide); };
     // About two workgroups a CU for the prefix and three for the own rows, whose lengths differ, with at
-    // least 4 tiles of 32 rows a split.
-    auto splits_of = [&](long long tiles, long long items, int per_cu) {
-        return (int)std::max<long long>(1, std::min((per_cu * cu + items - 1) / items, (tiles + 3) / 4));
+    // least 4 tiles of 32 rows a split: a workgroup's start and its partial cost about as much (32 query
+    // rows of 128 dims against 4001 rows take 26 us so, 31 us from 2 tiles on).  At head_dim 256 a CU holds one
+    // workgroup, whose tiles take several times as long: one a CU, from 1 and 2 tiles on (48 sequences
+    // of 4 heads against 5000 + 2000 rows: 45 us, 56 us with two and three a CU; 12 of 9 tokens against
+    // 300 + 900: 20 us, 31 us from 4 tiles on).
+    const bool one = head_dim > 128;
+    auto splits_of = [&](long long tiles, long long items, int per_cu, int least) {
+        return (int)std::max<long long>(1, std::min((per_cu * cu + items - 1) / items, (tiles + least - 1) / least));
     };
     PagedPlan p{};
     const long long each = (rows + n_seqs - 1) / n_seqs;
@@ -158,11 +163,12 @@ inline PagedPlan paged_plan(int n_seqs, int n_tokens, int n_heads, int n_kv_head
     p.own_wide = wide_of(each);
     if (prefix > 0) {
         const long long tiles = (prefix + 31) / 32;
-        const int s = splits_of(tiles, items_of(rows, p.prefix_wide) * n_kv_heads, 2);
+        const int s = splits_of(tiles, items_of(rows, p.prefix_wide) * n_kv_heads, one ? 1 : 2, one ? 1 : 4);
         p.prefix_tiles = (int)((tiles + s - 1) / s);
         p.prefix_splits = (int)((tiles + p.prefix_tiles - 1) / p.prefix_tiles);
     }
-    p.own_splits = splits_of((std::max(max_len - prefix, 1) + 31) / 32, n_seqs * items_of(each, p.own_wide) * n_kv_heads, 3);
+    p.own_splits = splits_of((std::max(max_len - prefix, 1) + 31) / 32, n_seqs * items_of(each, p.own_wide) * n_kv_heads,
+                             one ? 1 : 3, one ? 2 : 4);
     return p;
 }
 
