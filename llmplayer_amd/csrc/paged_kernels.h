@@ -5,6 +5,8 @@
 #include "paged_args.h"
 #include "prefill_kernels.h"
 
+#include <type_traits>
+
 namespace llmp {
 namespace pg {
 
@@ -18,7 +20,27 @@ typedef pk::floatx4 floatx4;
 //   in the same order; seq_start is the exclusive sum of the new tokens, and token i of sequence b
 //   has position len_b + i and slot blocks[b][pos / P] * P + pos % P.
 constexpr int kTablesThreads = 1024;
+constexpr int kTablesPer = kTablesMaxSeqs / kTablesThreads;   // sequences of a thread, at most
 inline size_t tables_lds(int n) { return ((size_t)n * 4 + 3) * sizeof(int); }
+
+__device__ __forceinline__ unsigned add_capped(unsigned a, unsigned b) { return min(a + b, 0x7fffffffu); }   // both below 2^31
+// Inclusive sum over the wave's lanes, or over its rows of 16 each.
+template <bool ROW>
+__device__ __forceinline__ unsigned wave_scan(unsigned x) {
+    auto step = [&](auto ctrl, auto rows) {   // (0 comes in from outside the row and to masked rows)
+        x = add_capped(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+    };
+    using All = std::integral_constant<int, 0xF>;
+    step(std::integral_constant<int, 0x111>{}, All{});   // row_shr:1, 2, 4, 8
+    step(std::integral_constant<int, 0x112>{}, All{});
+    step(std::integral_constant<int, 0x114>{}, All{});
+    step(std::integral_constant<int, 0x118>{}, All{});
+    if constexpr (!ROW) {
+        step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});   // row_bcast:15 to rows 1 and 3
+        step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});   // row_bcast:31 to rows 2 and 3
+    }
+    return x;
+}
 
 // Every workgroup reads all lengths and forms the three exclusive sums itself (a few KB out of
 // L2), then takes its share of the tokens, blocks and returned pages: one launch, no exchange.
@@ -31,75 +53,82 @@ __global__ __launch_bounds__(kTablesThreads) void paged_tables_kernel(TablesArgs
     int* s_start = s_len + n;        // n + 1
     int* s_need = s_start + n + 1;   // n + 1
     int* s_back = s_need + n + 1;    // n + 1
-    __shared__ long long s_sum[3][kTablesThreads / 64];
+    __shared__ uint4 s_sum[kTablesThreads / 64];
     __shared__ int s_last;
     const int n_free = *a.n_free;
     const int P1 = (1 << a.shift) - 1;
-    int bad = n_free < 0 || n_free > a.n_pages;
-    for (int i = tid; i < n; i += kTablesThreads) {
-        const int l = a.len[i], g = a.grow[i];
-        const bool ended = g < 0;
-        const int add = ended ? 0 : g;
-        const bool wrong = l < 0 || (long long)l + add > a.max_seq;
+    // The thread's `per` consecutive sequences, all loads at once.
+    const int per = (n + kTablesThreads - 1) / kTablesThreads, i0 = tid * per;
+    int l[kTablesPer], grow[kTablesPer];
+#pragma unroll
+    for (int k = 0; k < kTablesPer; ++k) {
+        const int i = min(i0 + k, n - 1);
+        if (k < per) {
+            l[k] = a.len[i];
+            grow[k] = a.grow[i];
+        }
+    }
+    // New tokens, blocks to take and blocks given back: sums that stop at 2^31 - 1, above all that a step
+    // may hold.
+    unsigned bad = n_free < 0 || n_free > a.n_pages, own[3] = {0, 0, 0};
+    int need[kTablesPer], back[kTablesPer];
+#pragma unroll
+    for (int k = 0; k < kTablesPer; ++k) {
+        if (k >= per || i0 + k >= n) break;
+        const bool ended = grow[k] < 0;
+        const int add = ended ? 0 : grow[k];
+        const bool wrong = l[k] < 0 || (long long)l[k] + add > a.max_seq;
         bad |= wrong;
-        const int len = wrong ? 0 : l, grow = wrong ? 0 : add;
+        const int len = wrong ? 0 : l[k];
+        grow[k] = wrong ? 0 : add;
         const int have = (int)(((unsigned)len + P1) >> a.shift);
-        const int after = (int)(((unsigned)len + (unsigned)grow + P1) >> a.shift);
-        s_len[i] = ended ? ~len : len;
-        s_start[i] = grow;
-        s_need[i] = ended ? 0 : after - have;
-        s_back[i] = ended && !wrong ? max(have - a.shared, 0) : 0;
+        const int after = (int)(((unsigned)len + (unsigned)grow[k] + P1) >> a.shift);
+        need[k] = ended ? 0 : after - have;
+        back[k] = ended && !wrong ? max(have - a.shared, 0) : 0;
+        l[k] = ended ? ~len : len;
+        own[0] = add_capped(own[0], grow[k]);
+        own[1] = add_capped(own[1], need[k]);
+        own[2] = add_capped(own[2], back[k]);
     }
-    bad = __syncthreads_or(bad);
-    // Exclusive sums: each thread over its `per` consecutive sequences, the wave by shuffles, the
-    // waves through LDS.
-    const int per = (n + kTablesThreads - 1) / kTablesThreads;
-    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
-    long long own[3] = {0, 0, 0};
-    for (int i = i0; i < i1; ++i) {
-        own[0] += s_start[i];
-        own[1] += s_need[i];
-        own[2] += s_back[i];
-    }
-    long long at[3];
+    unsigned at[3], total[3];
+#pragma unroll
+    for (int q = 0; q < 3; ++q) at[q] = wave_scan<false>(own[q]);
+    bad = __ballot(bad != 0) != 0;
+    if (lane == 63) s_sum[wave] = make_uint4(at[0], at[1], at[2], bad);
+    __syncthreads();
+    const uint4 w = s_sum[lane & (kTablesThreads / 64 - 1)];
+    const unsigned part[3] = {w.x, w.y, w.z};
+    bad = __ballot(w.w != 0) != 0;
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
-        long long x = own[q];
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const long long y = __shfl_up(x, off);
-            if (lane >= off) x += y;
-        }
-        if (lane == 63) s_sum[q][wave] = x;
-        at[q] = x - own[q];
+        const unsigned sums = wave_scan<true>(part[q]);
+        total[q] = __builtin_amdgcn_readlane(sums, kTablesThreads / 64 - 1);
+        const unsigned before = __builtin_amdgcn_readlane(sums, max(__builtin_amdgcn_readfirstlane(wave) - 1, 0));
+        // (an inclusive sum less the thread's own; where sums were capped the step is refused)
+        at[q] = at[q] - own[q] + (wave > 0 ? before : 0);
     }
-    __syncthreads();
-    long long total[3] = {0, 0, 0};
-#pragma unroll
-    for (int q = 0; q < 3; ++q)
-        for (int w = 0; w < kTablesThreads / 64; ++w) {
-            if (w == wave) at[q] += total[q];
-            total[q] += s_sum[q][w];
-        }
     int status = 0;
-    if (bad || n_free + total[2] > a.n_pages) status = -1;
-    else if (total[0] > a.max_tokens) status = -2;
-    else if (total[1] > n_free + total[2]) status = (int)min(total[1] - n_free - total[2], (long long)0x7fffffff);
+    if (bad || (long long)n_free + total[2] > a.n_pages) status = -1;
+    else if (total[0] > (unsigned)a.max_tokens) status = -2;
+    else if (total[1] > n_free + total[2]) status = (int)(total[1] - n_free - total[2]);
     const bool good = status == 0;
-    for (int i = i0; i < i1; ++i) {   // the thread's own entries: no other thread reads them yet
-        const int x = s_start[i], y = s_need[i], z = s_back[i];
+#pragma unroll
+    for (int k = 0; k < kTablesPer; ++k) {
+        const int i = i0 + k;
+        if (k >= per || i >= n) break;
+        s_len[i] = l[k];
         s_start[i] = good ? (int)at[0] : 0;
         s_need[i] = good ? (int)at[1] : 0;
         s_back[i] = good ? (int)at[2] : 0;
-        at[0] += x;
-        at[1] += y;
-        at[2] += z;
+        at[0] += grow[k];
+        at[1] += need[k];
+        at[2] += back[k];
     }
-    const int tokens = good ? (int)total[0] : 0, need = good ? (int)total[1] : 0, back = good ? (int)total[2] : 0;
+    const int tokens = good ? (int)total[0] : 0, taken = good ? (int)total[1] : 0, given = good ? (int)total[2] : 0;
     if (tid == 0) {
         s_start[n] = tokens;
-        s_need[n] = need;
-        s_back[n] = back;
+        s_need[n] = taken;
+        s_back[n] = given;
     }
     __syncthreads();
     // All inputs of this workgroup are in LDS and registers: the last workgroup to come here may write over
@@ -108,7 +137,7 @@ __global__ __launch_bounds__(kTablesThreads) void paged_tables_kernel(TablesArgs
     int ticket = 0;
     if (tid == 0 && gridDim.x > 1) ticket = atomicAdd(a.ticket, 1);
     // Entry e of the stack after the pushes, as the popping tokens see it.
-    const int top = n_free + back;
+    const int top = n_free + given;
     auto returned = [&](int r) {
         const int b = paged_owner(s_back, n, r);
         return a.blocks[(long long)b * a.width + a.shared + (r - s_back[b])];
@@ -132,12 +161,12 @@ __global__ __launch_bounds__(kTablesThreads) void paged_tables_kernel(TablesArgs
         a.positions[i] = pos;
         a.slots[i] = slot;
     }
-    for (int r = g0; r < need; r += gn) {
+    for (int r = g0; r < taken; r += gn) {
         const int b = paged_owner(s_need, n, r);
         const int have = (int)(((unsigned)s_len[b] + P1) >> a.shift);
         a.blocks[(long long)b * a.width + have + (r - s_need[b])] = popped(r);
     }
-    for (int r = g0; r < back; r += gn) a.free_pages[n_free + r] = returned(r);
+    for (int r = g0; r < given; r += gn) a.free_pages[n_free + r] = returned(r);
     if (blockIdx.x == 0 && tid == 0) *a.status = status;
     if (tid == 0) {
         s_last = gridDim.x == 1 || ticket == (int)gridDim.x - 1;
@@ -152,7 +181,7 @@ __global__ __launch_bounds__(kTablesThreads) void paged_tables_kernel(TablesArgs
             if (good) a.len_out[i] = ended ? 0 : l + (s_start[i + 1] - s_start[i]);
             else if (a.len_out != a.len) a.len_out[i] = a.len[i];
         }
-        if (tid == 0) *a.n_free_out = good ? top - need : n_free;
+        if (tid == 0) *a.n_free_out = good ? top - taken : n_free;
     }
 }
 
