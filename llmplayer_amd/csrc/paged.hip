@@ -49,7 +49,7 @@ hipError_t launch_paged_tables(const pg::TablesArgs& a, hipStream_t st) {
     static const hipError_t allowed = allow_lds(pg::paged_tables_kernel, pg::tables_lds(kTablesMaxSeqs));
     if (allowed != hipSuccess) return allowed;
     const long long work = std::max<long long>(a.max_tokens, 8LL * a.n);
-    const int wgs = (int)std::min<long long>(64, (work + pg::kTablesThreads - 1) / pg::kTablesThreads);
+    const int wgs = (int)std::min<long long>(256, (work + pg::kTablesThreads - 1) / pg::kTablesThreads);
     hipLaunchKernelGGL(pg::paged_tables_kernel, dim3(std::max(wgs, 1)), dim3(pg::kTablesThreads), pg::tables_lds(a.n), st, a);
     return hipGetLastError();
 }

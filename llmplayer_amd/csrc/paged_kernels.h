@@ -45,7 +45,9 @@ __device__ __forceinline__ unsigned wave_scan(unsigned x) {
 // Every workgroup reads all lengths and forms the three exclusive sums itself (a few KB out of
 // L2), then takes its share of the tokens, blocks and returned pages: one launch, no exchange.
 // len_out and n_free_out may lie over the inputs, so the workgroup that is last to have read them
-// writes both.  Bound by latency: three dependent memory trips and the scan's barriers.
+// writes both.  Bound by latency: the start, three dependent memory trips, the sums' barriers and, with
+// thousands of sequences, the search of a token's one (48 sequences of one token: 4.6 us; 300 with
+// prompts of up to 900: 7.1 us, with 64 workgroups in place of 256 8.8 us; 4096 of 4 tokens: 10.5 us).
 __global__ __launch_bounds__(kTablesThreads) void paged_tables_kernel(TablesArgs a) {
     extern __shared__ int s_dyn[];
     const int n = a.n, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
