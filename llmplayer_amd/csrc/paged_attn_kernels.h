@@ -549,7 +549,11 @@ __device__ __forceinline__ void store_part(const AttnArgs& a, const ItemRows& x,
 }
 
 // 16 query rows against a split of the prefix, or (OWN) of one sequence's own rows; the waves take the
-// split's tiles in turn.
+// split's tiles in turn.  Bound by memory latency: two waves per SIMD are all that K and V of a tile in
+// registers leave, each with one tile on its way (one token of 32 sequences, 32 + 8 heads of 128, up to 1500 own fp32
+// rows each: 50 us, 3.8 TB/s; 64 sequences, 32 + 8 heads of 64, up to 2000 Q8_0 rows: 40 us, where the split
+// of the quants takes 17 us of every SIMD).  The four query heads of such a KV head fill a quarter of the 16 rows: the
+// matrix units run 5 to 10 % of the time, so no smaller tile is made for them.
 template <int D, bool Q8, bool OWN>
 __device__ __forceinline__ void attn_narrow(const AttnArgs& a, uint4* lds, int item, int h, int split) {
     using T = Tile<D, Q8>;
@@ -916,7 +920,13 @@ struct TilePart {
 
 // 64*MT query rows, 16*MT a wave, against a split of the prefix, or (OWN) of one sequence's own rows.
 // Two tiles in LDS (one at head_dim 256, whose two would leave room for one workgroup a CU): while the
-// waves multiply tile i, they hold tile i + 2 in flight and have stored i + 1.
+// waves multiply tile i, they hold tile i + 2 in flight and have stored i + 1: one barrier a tile (an item of 128
+// rows against 32001 shared rows of 128 dims: 109 us with one tile and two barriers, 84 us, 3.1 TB/s).
+// Many rows are bound by the vector units: of each SIMD's 340 us in 12 prompts of up to 700 tokens, 32 + 8 heads of
+// 64, behind 2000 shared rows (235 TFLOP/s, three times that in fp16 products), they take 155, the matrix units 91:
+// exponentials, the split of P, the split of K and V, which 128 rows share (with 64 rows an item 430 us in place of
+// 310).  Few rows against a long prefix are bound by the latency of one tile in flight per workgroup; 64
+// rows an item read each tile twice and take 107 us where 128 take 93.
 template <int D, int MT, bool Q8, bool OWN>
 __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int item, int h, int split) {
     using T = TilePart<D, Q8>;
@@ -1207,7 +1217,9 @@ __global__ __launch_bounds__(kAttnThreads, D > 128 ? 1 : 2) void paged_attn_kern
     }
 }
 
-// Joins the partials of each query row (prefix splits, then own splits) and applies sink and gate.  A
+// Joins the partials of each query row (prefix splits, then own splits) and applies sink and gate.  Bound by
+// memory where there are many rows (4700 tokens of 32 heads of 64, two partials: 17 us, 6.5 TB/s), by its
+// start where there are few (3 to 5 us).  A
 // group of D/4 threads (four dims each) takes one row's partials; a row with several of them is taken by
 // GR groups, every GR-th partial each, all loads in flight together, which meet in LDS in a fixed
 // order.  A row with nothing to attend is zero; rows of tokens behind the last sequence are left as they

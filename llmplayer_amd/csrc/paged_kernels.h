@@ -356,9 +356,10 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(AppendArgs
     }
 }
 
-// The others (sequential norms, odd strides, blocks that do not lie in whole lanes).  One workgroup = (token, group of kAppendHeads heads): the heads [h0, h0 + kAppendHeads) of the token's
-// query, key and value heads in that order, staged in LDS and prepared with the decode path's
-// functions, so the rows are bit-identical to a decode append's (before they are quantised).
+// The others (sequential norms, odd strides, blocks that do not lie in whole lanes).  One workgroup = (token,
+// group of kAppendHeads heads): the heads [h0, h0 + kAppendHeads) of the token's query, key and value
+// heads in that order, staged in LDS and prepared with the decode path's functions, so the rows are
+// bit-identical to a decode append's (before they are quantised).
 constexpr int kAppendHeads = 8;
 template <int D>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_lds_kernel(AppendArgs a) {
