@@ -480,8 +480,9 @@ int llmp_paged_tables(uint64_t handle, int n_seqs, int shared_blocks, int max_to
  * rounded as there, with block scales max|x| * (1/127) (a product where a contiguous cache divides:
  * one unit in the last place at most).
  * k = v = 0: only the queries (slots may be 0).  in_type: the type of q, k and v (LLMP_IN_*); strides
- * in elements, at least a row; q_out may be q for fp32 at equal strides.  A token with no position is
- * skipped, its q_out row too.  No two tokens may name one slot. */
+ * in elements, at least a row; q_out may be q for fp32 at equal strides, and shares no element with q, k
+ * or v otherwise.  A token with no position is skipped, its q_out row too.  No two tokens may name one
+ * slot. */
 #define LLMP_IN_F32  0
 #define LLMP_IN_BF16 1
 int llmp_paged_append(uint64_t handle, int layer, int n_tokens, uint64_t positions, uint64_t slots,

@@ -281,3 +281,90 @@ def test_rows_far_into_a_large_pool():
                 b.check(d.down(out, F32, (3, hq, D)), *b.want(), what=f"large pool, cache {cache}")
             finally:
                 kv.destroy()
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_drawn(seed):
+    """Every shape, cache, page and mask with every other, up to prompts that take items of 128 rows."""
+    rng = np.random.default_rng(1000 + seed)
+    hq, hkv, D = SHAPES[rng.integers(len(SHAPES))]
+    n = int(rng.choice([1, 2, 3, 9, 30]))
+    most = int(rng.choice([1, 1, 4, 40, 130])) if n < 30 else 2
+    prefix = int(rng.choice([0, 1, 47, 64, 200, 777]))
+    held = rng.integers(0, int(rng.choice([1, 40, 600])), n).tolist()
+    new = rng.integers(0, most + 1, n).tolist()
+    new[int(rng.integers(n))] = most
+    b = Batch(rng, hq, hkv, D, int(rng.choice([16, 32, 64, 128, 256])), prefix, held, new, cache=int(rng.integers(3)),
+              window=int(rng.choice([0, 0, 0, 1, 50, 300])), pad=int(rng.integers(3)),
+              garbage=str(rng.choice(["nan", "inf", "huge"])))
+    kw = {}
+    if rng.random() < 0.3:
+        kw["scale"] = 0.2
+    if rng.random() < 0.3:
+        kw["softcap"] = 10.0
+    if rng.random() < 0.3:
+        kw["sinks"] = rng.standard_normal(hq).astype(F32)
+    if rng.random() < 0.3:
+        kw["gate"] = rng.standard_normal((b.n_tokens, hq, D)).astype(F32)
+    if rng.random() < 0.25:     # tokens anywhere in their sequences, and none
+        positions = b.positions.copy()
+        for s, t in enumerate(b.total):
+            for i in range(b.seq_start[s], b.seq_start[s + 1]):
+                positions[i] = rng.integers(-1, t)
+        kw["positions"] = positions
+    if rng.random() < 0.25:     # blocks that no page holds
+        blocks = b.blocks.copy()
+        blocks[rng.random(blocks.shape) < 0.1] = rng.choice([-1, b.n_pages, 2 ** 31 - 1, -2 ** 31])
+        kw["blocks"] = blocks
+    with pc.Device() as d:
+        got = b.run(d, strides=4 * int(rng.integers(3)), max_len=int(rng.choice([0, 1, b.max_seq])), **kw)
+        b.check(got, *b.want(**kw), what=f"seed {seed}: {hq}/{hkv}/{D} n {n} new {most} prefix {prefix} cache {b.cache} {sorted(kw)}")
+
+
+@pytest.mark.parametrize("cache", [0, 1], ids=["f32", "q8"])
+@pytest.mark.parametrize("hq,hkv,D", [(8, 2, 64), (8, 2, 96), (8, 2, 128), (4, 1, 256)])
+def test_a_bad_row_among_many_queries(hq, hkv, D, cache):
+    """Row 75 of a prompt of 150 tokens: the tokens before it stay what they were."""
+    rng = rng_of(hq, D, cache, 30)
+    b = Batch(rng, hq, hkv, D, 32, 45, [0, 10], [150, 90], cache)
+    want, tol = b.want()
+    p = 45 + 75
+    for w in (("k", "v") if cache == 0 else ("ks", "vs")):
+        for value in (np.nan, np.inf):
+            plane = b.planes[w]
+            kept = plane.copy()
+            plane[b.blocks[0][p // 32], :, p % 32, 0] = value
+            with pc.Device() as d:
+                got = b.run(d)
+            b.planes[w][:] = kept
+            hit = slice(75, 150)
+            assert not np.isfinite(got[hit][..., 0]).any(), (w, value)
+            y = want.copy()
+            got[hit], y[hit] = 0, 0
+            b.check(got, y, tol, what=f"{value} in {w}")
+
+
+def test_other_streams():
+    """The same call on a stream of its own, and twice on one handle in turn on two streams."""
+    import ctypes as C
+    rng = rng_of(31)
+    b = Batch(rng, 8, 2, 128, 16, 300, [0, 90, 5], [1, 3, 60])
+    kv = PagedKv(1, b.n_pages, b.page, b.max_seq, b.hkv, b.D, 0)
+    streams = [C.c_uint64() for _ in range(2)]
+    try:
+        for s in streams:
+            _lib.call("llmp_stream_create", C.byref(s))
+        with pc.Device() as d:
+            first = b.run(d, kv=kv)
+            b.check(first, *b.want(), what="library stream")
+            for s in streams + streams:
+                out = d.up(np.full((b.n_tokens, b.hq * b.D), 77, F32))
+                args = list(b.args)
+                args[12], args[14] = out, s.value
+                _lib.call("llmp_paged_attn", *args)
+                _lib.call("llmp_stream_sync", s.value)
+                assert np.array_equal(d.down(out, F32, first.shape).view(np.uint32), first.view(np.uint32))
+    finally:
+        for s in streams:
+            _lib.call("llmp_stream_destroy", s.value)
+        kv.destroy()
