@@ -127,6 +127,23 @@ def test_refused_steps_change_nothing(what, in_place):
             kv.destroy()
 
 
+@pytest.mark.parametrize("n", [4096, 4095])
+def test_sums_beyond_32_bits(n):
+    """2^20 new tokens of each of 4096 sequences: 2^32 of them."""
+    max_seq, page = 1 << 20, 256
+    c = {"length": np.zeros(n, I), "grow": np.full(n, 1 << 20, I), "free": np.arange(8, dtype=I), "n_free": 8,
+         "blocks": np.full((n, max_seq // page), -1, I), "n_pages": 8}
+    with pc.Device() as d:
+        kv = PagedKv(1, 8, page, max_seq, 1, 64)
+        try:
+            p, _ = run(d, kv, c, 0, 1000)
+            want = {"status": -2, "n_free": 8, "len": c["length"], "seq_start": np.zeros(n + 1, I), "positions": np.full(1000, -1, I),
+                    "slots": np.full(1000, -1, I), "blocks": c["blocks"], "free": c["free"]}
+            check(d, p, c, want, 1000, "2^32 tokens")
+        finally:
+            kv.destroy()
+
+
 def test_entries_outside_the_pool_give_no_slot():
     c = {"length": np.array([20, 5], I), "grow": np.array([3, 1], I), "free": np.arange(6, dtype=I), "n_free": 4,
          "blocks": np.array([[4, 77, -1, -1], [-3, 0, 0, 0]], I), "n_pages": 6}
