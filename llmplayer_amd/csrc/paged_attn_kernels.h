@@ -733,53 +733,51 @@ __device__ __forceinline__ void attn_narrow(const AttnArgs& a, uint4* lds, int i
 // ---- a tile shared by four waves ---------------------------------------------------------------
 // Rows of it: 64 at head_dim 64, 32 above (the same bytes).  In LDS: K as [16-row parts x D/32 steps][hi,
 // lo][lane] and V as [32-row groups x D/16 output tiles][hi, lo][lane], 16 bytes a lane, exactly the
-// operands: every read is one conflict-free b128.  A wave loads, cleans and splits the K operands
-// p = wave, wave + 4, ... and the V units (64 dims, 16-row part) likewise; a unit's lane holds 4 rows of 4
-// dims, 8 bytes of four operands.
+// operands: every read is one conflict-free b128.  A wave loads, cleans and splits operands of K and units
+// of V (64 dims) of one 16-row part, so that one entry of the block table serves all of its loads; a unit's lane
+// holds 4 rows of 4 dims, 8 bytes of four operands.
 constexpr int wide_rows(int D) { return D == 64 ? 64 : 32; }
 constexpr int wide_tiles(int D) { return D <= 128 ? 2 : 1; }
 
 template <int D, bool Q8>
 struct TilePart {
     static constexpr int KS = D / 32, NC = D / 64, REM = D % 64 / 32, DT = D / 16, NU = wide_rows(D) / 16;
-    static constexpr int NK = NU * KS, NV = NU * (NC + REM);
-    static constexpr int KP = (NK + 3) / 4, VP = (NV + 3) / 4;
+    static constexpr int NK = NU * KS, NV = NC + REM, WPP = 4 / NU;   // WPP: waves of a part
+    static constexpr int KP = (KS + WPP - 1) / WPP, VP = (NV + WPP - 1) / WPP;
     static constexpr int kBytes = (NK + NU / 2 * DT) * 2 * 64 * 16;
     floatx4 k[KP][2];      // Q8: 8 quants in the first two words, the scale in the third
     floatx4 v[VP][4];      // Q8: 4 quants and their scale
 
-    // The 16-row part of K operand q and of V unit q, and its 64 dims.
-    static __device__ __forceinline__ int k_part(int q) { return q / KS; }
-    static __device__ __forceinline__ int v_part(int q) { return q % NU; }
-    static __device__ __forceinline__ int v_dims(int q) { return q / NU; }
+    // The wave's 16-row part; step s of its K operand i, and 64 dims c of its V unit i.
+    static __device__ __forceinline__ int part(int wave) { return wave / WPP; }
+    static __device__ __forceinline__ int k_step(int wave, int i) { return KP * (wave % WPP) + i; }
+    static __device__ __forceinline__ int v_dims(int wave, int i) { return VP * (wave % WPP) + i; }
+    static __device__ __forceinline__ bool no_k(int wave, int i) { return KS % WPP != 0 && k_step(wave, i) >= KS; }
+    static __device__ __forceinline__ bool no_v(int wave, int i) { return NV % WPP != 0 && v_dims(wave, i) >= NV; }
 
-    // The pages of the wave's parts (kp, vp), and row(u): the first row in its page of 16-row part u.
-    template <class Row>
-    __device__ __forceinline__ void load(const PoolPlanes& p, const int (&kp)[KP], const int (&vp)[VP], const Row& row, int h,
-                                         int wave, int n, int g) {
+    // From row `row` of `page` on.
+    __device__ __forceinline__ void load(const PoolPlanes& p, int page, int row, int h, int wave, int n, int g) {
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            const int q = wave + 4 * i;
-            if (NK % 4 != 0 && q >= NK) break;
-            const int u = k_part(q), s = q % KS;
+            if (no_k(wave, i)) break;
+            const int s = k_step(wave, i);
             if constexpr (Q8) {
-                const uint2 w = at<uint2>(page_rows(p.k, p, kp[i], h, row(u), D) + 32 * s, D * n + 8 * g);
+                const uint2 w = at<uint2>(page_rows(p.k, p, page, h, row, D) + 32 * s, D * n + 8 * g);
                 k[i][0] = floatx4{__uint_as_float(w.x), __uint_as_float(w.y),
-                                  at<float>(page_rows(p.ks, p, kp[i], h, row(u), 4 * KS) + 4 * s, 4 * KS * n), 0};
+                                  at<float>(page_rows(p.ks, p, page, h, row, 4 * KS) + 4 * s, 4 * KS * n), 0};
             } else {
-                const char* b = page_rows(p.k, p, kp[i], h, row(u), 4 * D) + 128 * s;
+                const char* b = page_rows(p.k, p, page, h, row, 4 * D) + 128 * s;
                 k[i][0] = at<floatx4>(b, 4 * D * n + 32 * g);
                 k[i][1] = at<floatx4>(b, 4 * D * n + 32 * g + 16);
             }
         }
 #pragma unroll
         for (int i = 0; i < VP; ++i) {
-            const int q = wave + 4 * i;
-            if (NV % 4 != 0 && q >= NV) break;
-            const int u = v_part(q), c = v_dims(q);
+            if (no_v(wave, i)) break;
+            const int c = v_dims(wave, i);
             if constexpr (Q8) {
-                const char* b = page_rows(p.v, p, vp[i], h, row(u), D) + 64 * c;
-                const char* sc = page_rows(p.vs, p, vp[i], h, row(u), 4 * KS) + 8 * c;
+                const char* b = page_rows(p.v, p, page, h, row, D) + 64 * c;
+                const char* sc = page_rows(p.vs, p, page, h, row, 4 * KS) + 8 * c;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const unsigned r = 4 * g + j;
@@ -788,7 +786,7 @@ struct TilePart {
                     v[i][j] = floatx4{__uint_as_float(w), at<float>(sc, 4 * KS * r + (full ? 4 * (n >> 3) : 0)), 0, 0};
                 }
             } else {
-                const char* b = page_rows(p.v, p, vp[i], h, row(u), 4 * D) + 256 * c;
+                const char* b = page_rows(p.v, p, page, h, row, 4 * D) + 256 * c;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const unsigned r = 4 * D * (4 * g + j);
@@ -810,9 +808,8 @@ struct TilePart {
         unsigned long long bad = 0;
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            const int q = wave + 4 * i;
-            if (NK % 4 != 0 && q >= NK) break;
-            const int row = 16 * k_part(q) + n;
+            if (no_k(wave, i)) break;
+            const int row = 16 * part(wave) + n;
             const unsigned keep = 0u - (unsigned)held(row);
             unsigned worst = 0;
             if constexpr (Q8) {
@@ -825,11 +822,10 @@ struct TilePart {
         }
 #pragma unroll
         for (int i = 0; i < VP; ++i) {
-            const int q = wave + 4 * i;
-            if (NV % 4 != 0 && q >= NV) break;
+            if (no_v(wave, i)) break;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int row = 16 * v_part(q) + 4 * g + j;
+                const int row = 16 * part(wave) + 4 * g + j;
                 const unsigned keep = 0u - (unsigned)held(row);
                 unsigned worst = 0;
                 if constexpr (Q8) {
@@ -848,7 +844,7 @@ struct TilePart {
         float x = 0.0f, y = 0.0f;
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            if (NK % 4 != 0 && wave + 4 * i >= NK) break;
+            if (no_k(wave, i)) break;
             if constexpr (Q8) {
                 x = max_abs(x, k[i][0][2], k[i][0][2]);
             } else {
@@ -858,7 +854,7 @@ struct TilePart {
         }
 #pragma unroll
         for (int i = 0; i < VP; ++i) {
-            if (NV % 4 != 0 && wave + 4 * i >= NV) break;
+            if (no_v(wave, i)) break;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (Q8) {
@@ -877,8 +873,8 @@ struct TilePart {
     __device__ __forceinline__ void store(uint4* lds, float fk, float fv, int wave, int lane) const {
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            const int q = wave + 4 * i;
-            if (NK % 4 != 0 && q >= NK) break;
+            if (no_k(wave, i)) break;
+            const int q = part(wave) * KS + k_step(wave, i);
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = Q8 ? quant(k[i][0][e >> 2], e & 3) : k[i][e >> 2][e & 3];
@@ -890,9 +886,8 @@ struct TilePart {
         uint2* lv = reinterpret_cast<uint2*>(lds + NK * 2 * 64);
 #pragma unroll
         for (int i = 0; i < VP; ++i) {
-            const int q = wave + 4 * i;
-            if (NV % 4 != 0 && q >= NV) break;
-            const int u = v_part(q), c = v_dims(q);
+            if (no_v(wave, i)) break;
+            const int u = part(wave), c = v_dims(wave, i);
 #pragma unroll
             for (int t = 0; t < 4; t += 2) {   // columns t and t + 1
                 if (REM && c >= NC && t > 0) break;
@@ -993,47 +988,21 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
     // pool holds no rows (page 0 is read instead and masked).
     auto entry = [&](int tile, int u) { return x.blk[min((row0 + tile * TR + 16 * u) >> a.pool.shift, a.width - 1)]; };
     auto in_pool = [&](int e) { return paged_page_ok(e, a.pool.n_pages); };
-    // The loaded tile t, its pages' entries c, and the next one's e: of the wave's parts.
+    // The loaded tile t, the entry c of the wave's part of it, and the next tile's e.
     T t;
-    int ek[T::KP] = {}, ev_[T::VP] = {}, ck[T::KP] = {}, cv[T::VP] = {};
-    auto entries = [&](int tile) {
-#pragma unroll
-        for (int i = 0; i < T::KP; ++i) ek[i] = entry(tile, T::k_part(wave + 4 * i));
-#pragma unroll
-        for (int i = 0; i < T::VP; ++i) ev_[i] = entry(tile, T::v_part(wave + 4 * i));
-    };
+    int e = 0, c = 0;
+    const int part = T::part(wave);
     auto load = [&](int tile) {
-        int pk_[T::KP], pv_[T::VP];
-#pragma unroll
-        for (int i = 0; i < T::KP; ++i) {
-            ck[i] = __builtin_amdgcn_readfirstlane(ek[i]);
-            pk_[i] = in_pool(ck[i]) ? ck[i] : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < T::VP; ++i) {
-            cv[i] = __builtin_amdgcn_readfirstlane(ev_[i]);
-            pv_[i] = in_pool(cv[i]) ? cv[i] : 0;
-        }
-        entries(tile + 1);
-        t.load(a.pool, pk_, pv_, [&](int u) { return (row0 + tile * TR + 16 * u) & rmask; }, h, wave, n, g);
-    };
-    // Parts of the loaded tile that no page of the pool holds, of those that the wave loads.
-    auto parts_gone = [&]() {
-        unsigned y = 0;
-#pragma unroll
-        for (int i = 0; i < T::KP; ++i)
-            if (T::NK % 4 == 0 || wave + 4 * i < T::NK) y |= (unsigned)!in_pool(ck[i]) << T::k_part(wave + 4 * i);
-#pragma unroll
-        for (int i = 0; i < T::VP; ++i)
-            if (T::NV % 4 == 0 || wave + 4 * i < T::NV) y |= (unsigned)!in_pool(cv[i]) << T::v_part(wave + 4 * i);
-        return y;
+        c = __builtin_amdgcn_readfirstlane(e);
+        e = entry(tile + 1, part);
+        t.load(a.pool, in_pool(c) ? c : 0, (row0 + tile * TR + 16 * part) & rmask, h, wave, n, g);
     };
     auto held = [&](int k0, unsigned gone, int row) { return !(gone >> (row >> 4) & 1) && k0 + row >= lo && k0 + row < hi; };
     // The loaded tile's largest values, for the exponents; and where some query does not attend all of
     // it, or a value is infinite, what is not to be multiplied is taken out.
     auto inspect = [&](int tile) {
         const int k0 = row0 + tile * TR;
-        const unsigned gone = parts_gone();
+        const unsigned gone = (unsigned)!in_pool(c) << part;   // parts of it that no page of the pool holds: the wave's
         unsigned long long bad = 0;
         unsigned mx = t.largest(wave);
         const bool every = k0 >= max(lo, lo_every) && k0 + TR <= min(hi, hi_every) && gone == 0;
@@ -1134,7 +1103,7 @@ __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int ite
         }
     };
     if (tiles > 0) {
-        entries(0);
+        e = entry(0, part);
         load(0);
         inspect(0);
     }
