@@ -917,11 +917,11 @@ struct TilePart {
 // Two tiles in LDS (one at head_dim 256, whose two would leave room for one workgroup a CU): while the
 // waves multiply tile i, they hold tile i + 2 in flight and have stored i + 1: one barrier a tile (an item of 128
 // rows against 32001 shared rows of 128 dims: 109 us with one tile and two barriers, 84 us, 3.1 TB/s).
-// Many rows are bound by the vector units: of each SIMD's 340 us in 12 prompts of up to 700 tokens, 32 + 8 heads of
-// 64, behind 2000 shared rows (235 TFLOP/s, three times that in fp16 products), they take 155, the matrix units 91:
-// exponentials, the split of P, the split of K and V, which 128 rows share (with 64 rows an item 430 us in place of
-// 310).  Few rows against a long prefix are bound by the latency of one tile in flight per workgroup; 64
-// rows an item read each tile twice and take 107 us where 128 take 93.
+// Many rows are bound by the issue of two waves a SIMD: of its 340 us in 12 prompts of up to 700 tokens, 32 + 8
+// heads of 64, behind 2000 shared rows (300 us a call unprofiled, 240 TFLOP/s, three times that in fp16
+// products), vector instructions take 155, the matrix units 91: exponentials, the split of P, and the split of K and
+// V, which 128 rows share (with 64 rows an item 430 us).  Few rows against a long prefix are bound by the latency of
+// one tile in flight per workgroup; 64 rows an item read each tile twice and take 107 us where 128 take 90.
 template <int D, int MT, bool Q8, bool OWN>
 __device__ __forceinline__ void attn_wide(const AttnArgs& a, uint4* lds, int item, int h, int split) {
     using T = TilePart<D, Q8>;
